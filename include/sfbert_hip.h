@@ -640,6 +640,65 @@ int sfb_gemm_nt(sfb_stream_t stream, float* c, const void* a, const void* w, int
 int sfb_softmax_cross_entropy(sfb_stream_t stream, float* loss, float* row_loss, float* d_logits,
                               const float* logits, const int32_t* labels, uint64_t rows, uint32_t vocab);
 
+/* ---- operators on rows of logits (MI355X additions, no counterpart in the reference) --------------------------- */
+
+/* Shared by the four entry points below.  logits [dev] is rows x vocab of dtype (SFB_F32 or SFB_BF16), 16-byte aligned,
+ * with rows row_stride >= vocab elements apart (any stride: rows may start at any element; columns from vocab on are
+ * neither read nor written); d_logits has the same type, stride and alignment and may be logits itself.  Every result
+ * is a function of scale * logits (scale = 1 / temperature, SFB_LOGIT_SCALE_MIN .. SFB_LOGIT_SCALE_MAX), computed in
+ * fp32; bf16 gradients are rounded once.  -inf is a masked logit: probability 0, no share of the entropy, gradient 0.
+ * A row that holds NaN or +inf gives NaN, a row of nothing but -inf gives log probabilities of -inf, entropy 0 and a
+ * zero gradient.  Logits as large as the type's largest and lowest value are ordinary numbers.  Results of one launch
+ * do not depend on the order in which threads run: the same inputs give the same bits.
+ * stats [dev] float[rows][2] (may be NULL): the row's reference logit m and log2 sum_j 2^((x_j - m) scale log2(e)),
+ * which the backward entry points take; with s = scale, ln sum_j exp(s x_j) = s m + ln(2) stats[1].
+ * workspace [dev] 16-byte aligned, SFB_LOGIT_WORKSPACE_BYTES bytes, zero-filled once before its first use and left
+ * ready for the next launch, or NULL: with it, few long rows are each cut over several work-groups.  Launches that
+ * share a workspace must be ordered on one stream (graphs captured with one are replayed one after the other). */
+#define SFB_LOGIT_SCALE_MIN 1e-4f
+#define SFB_LOGIT_SCALE_MAX 1e4f
+#define SFB_LOGIT_WORKSPACE_BYTES (1u << 20)
+
+/* Log probabilities of given tokens, with entropy and top alternatives, of every row:
+ *   logprob[r][i] = scale x[tokens[r][i]] - ln sum_j exp(scale x_j)    (n_tokens <= 256 per row; 0 for a token outside
+ *                                                                       [0, vocab), which names no column)
+ *   entropy[r]    = - sum_j p_j ln p_j                                  (NULL: not computed)
+ *   top_ids[r], top_logprobs[r]: the top_k <= 64 largest logits, falling; of equal ones the lowest index first (-0 and
+ *                   +0 are equal, NaN stands above everything)
+ * n_tokens = 0 (tokens and logprob NULL) and top_k = 0 (top_ids and top_logprobs NULL) leave those out. */
+int sfb_token_logprobs(sfb_stream_t stream, float* logprob, float* entropy, float* stats, int32_t* top_ids,
+                       float* top_logprobs, const void* logits, int dtype, const int32_t* tokens, uint64_t rows,
+                       uint32_t vocab, uint64_t row_stride, uint32_t n_tokens, uint32_t top_k, float scale,
+                       void* workspace, size_t workspace_bytes);
+/* Gradient of sum_r ( sum_i d_logprob[r][i] logprob[r][i] + d_entropy[r] entropy[r] ):
+ *   d_logits[r][j] = scale ( sum_{i: tokens[r][i] = j} d_logprob[r][i] - p_j sum_i d_logprob[r][i]
+ *                            - d_entropy[r] p_j (ln p_j + entropy[r]) )
+ * over the tokens inside [0, vocab).  stats and entropy are what sfb_token_logprobs wrote; d_entropy NULL: no entropy
+ * term (entropy may then be NULL).  A row whose coefficients are all zero gets zeros, whatever its logits hold. */
+int sfb_token_logprobs_backward(sfb_stream_t stream, void* d_logits, const void* logits, int dtype,
+                                const int32_t* tokens, const float* stats, const float* entropy, const float* d_logprob,
+                                const float* d_entropy, uint64_t rows, uint32_t vocab, uint64_t row_stride,
+                                uint32_t n_tokens, float scale);
+/* Distillation from a teacher's top logits.  teacher_ids, teacher_logits [dev] [rows][slots] (slots <= 256; logits of
+ * teacher_dtype SFB_F32 or SFB_BF16): the tokens a teacher ranks highest and their logits, in any order; a slot whose
+ * id is outside [0, vocab) is unused (lists of different lengths).  With q = softmax(scale * teacher_logits) over a
+ * row's used slots and p = softmax(scale * logits) over the vocabulary,
+ *   row_loss[r] = 1 / scale^2 sum_k q_k (ln q_k - ln p[teacher_ids[r][k]])
+ * (Kullback-Leibler divergence times the squared temperature).  A token named twice counts with both slots.  A row
+ * without a used slot has loss 0; its logits are not read.
+ * d_logits not NULL: also the gradient of sum_r d_loss[r] row_loss[r] (d_loss [dev] float[rows]),
+ *   d_logits[r][j] = d_loss[r] / scale ( p_j - sum_{k: teacher_ids[r][k] = j} q_k ),
+ * in the same call; zeros where d_loss[r] is zero or the row has no used slot. */
+int sfb_distillation_loss(sfb_stream_t stream, float* row_loss, float* stats, void* d_logits, const void* logits,
+                          int dtype, const int32_t* teacher_ids, const void* teacher_logits, int teacher_dtype,
+                          const float* d_loss, uint64_t rows, uint32_t vocab, uint64_t row_stride, uint32_t slots,
+                          float scale, void* workspace, size_t workspace_bytes);
+/* The gradient on its own, from the stats that sfb_distillation_loss wrote. */
+int sfb_distillation_loss_backward(sfb_stream_t stream, void* d_logits, const void* logits, int dtype,
+                                   const int32_t* teacher_ids, const void* teacher_logits, int teacher_dtype,
+                                   const float* stats, const float* d_loss, uint64_t rows, uint32_t vocab,
+                                   uint64_t row_stride, uint32_t slots, float scale);
+
 /* Weights of the whole model (transformer_inference_part.cpp:60-148): token embedding [vocab][state] (also the
  * logits matrix), position embedding [ctx][state], both fp32 [dev]; tok_embed_bf16 [dev] the token embedding
  * rounded to bf16 (needed when dtype is bf16, else may be NULL); layers: HOST array of n_layers structs of device

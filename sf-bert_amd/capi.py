@@ -82,6 +82,7 @@ EXPORTED = [
     "sfb_encoder_layer_forward_streamed",
     "sfb_encoder_layer_forward_pre_ln", "sfb_gemm_nt", "sfb_softmax_cross_entropy", "sfb_model_workspace_bytes",
     "sfb_model_forward",
+    "sfb_token_logprobs", "sfb_token_logprobs_backward", "sfb_distillation_loss", "sfb_distillation_loss_backward",
 ]
 
 
@@ -889,6 +890,177 @@ def softmax_cross_entropy(logits, labels, want_grad=False, in_place=False):
     return (loss, row_loss, d) if want_grad else (loss, row_loss)
 
 
+# ------------------------------------------------------------------------------------ rows of logits
+LOGIT_WORKSPACE_BYTES = 1 << 20
+_P, _U32, _U64, _INT = C.c_void_p, C.c_uint32, C.c_uint64, C.c_int
+_LOGIT_ARGS = {
+    "sfb_token_logprobs": [_P, _P, _P, _P, _P, _P, _P, _INT, _P, _U64, _U32, _U64, _U32, _U32, C.c_float, _P, C.c_size_t],
+    "sfb_token_logprobs_backward": [_P, _P, _P, _INT, _P, _P, _P, _P, _P, _U64, _U32, _U64, _U32, C.c_float],
+    "sfb_distillation_loss": [_P, _P, _P, _P, _P, _INT, _P, _P, _INT, _P, _U64, _U32, _U64, _U32, C.c_float, _P, C.c_size_t],
+    "sfb_distillation_loss_backward": [_P, _P, _P, _INT, _P, _P, _INT, _P, _P, _U64, _U32, _U64, _U32, C.c_float],
+}
+_logit_entries = {}
+
+
+def _logit_call(name, *args):
+    fn = _logit_entries.get(name)
+    if fn is None:   # with argument types plain numbers are converted without a ctypes object for each
+        fn = getattr(lib, name)
+        fn.argtypes = _LOGIT_ARGS[name]
+        _logit_entries[name] = fn
+    _check(fn(_stream(), *args), name)
+
+
+def _require_device(*tensors):
+    """Launches go to the current device: tensors of another one (or of the host) are refused."""
+    import torch
+    here = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device.index != here):
+            raise SfbError(8, "tensor on %s, current device cuda:%d" % (t.device, here))
+
+
+def _logit_rows(logits):
+    """(dtype code, rows, vocab, row stride) of a [rows, vocab] tensor whose rows may be further apart than vocab."""
+    if logits.dim() != 2:
+        raise SfbError(4, "logits of %d dimensions" % logits.dim())
+    rows, vocab = logits.shape
+    if rows == 0 or vocab == 0:
+        raise SfbError(4, "logits of shape %s" % (tuple(logits.shape),))
+    stride, step = logits.stride()
+    if rows == 1:
+        stride = max(stride, vocab)
+    if (step != 1 and vocab > 1) or stride < vocab:
+        raise SfbError(4, "logits with strides %s" % (logits.stride(),))
+    return _dtype_code(logits), rows, vocab, stride
+
+
+def _small(t, shape, dtype, what):
+    """Pointer of a contiguous tensor of the given shape and type (None: NULL)."""
+    if t is None:
+        return None
+    if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+        raise SfbError(4, "%s of shape %s, strides %s (expected %s)" % (what, tuple(t.shape), t.stride(), tuple(shape)))
+    if t.dtype != dtype:
+        raise SfbError(5, "%s of %s" % (what, t.dtype))
+    return t.data_ptr()
+
+
+def _like_logits(logits, stride, out):
+    import torch
+    if out is None:
+        rows, vocab = logits.shape
+        buffer = torch.empty((rows, stride), dtype=logits.dtype, device=logits.device)
+        return buffer if stride == vocab else buffer[:, :vocab]
+    if out.shape != logits.shape or out.dtype != logits.dtype or (out.stride() != logits.stride() and logits.shape[0] > 1) \
+            or (out.stride(1) != 1 and logits.shape[1] > 1):
+        raise SfbError(4, "out with shape %s, strides %s, %s: expected those of the logits" % (tuple(out.shape), out.stride(), out.dtype))
+    return out
+
+
+def _logit_workspace(workspace):
+    if workspace is None:
+        return None, 0
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+def token_logprobs(logits, tokens=None, top_k=0, scale=1.0, entropy=False, workspace=None):
+    """Log probabilities under softmax(scale * logits) of given tokens, with entropy and top alternatives
+    (sfb_token_logprobs).  logits [rows, vocab] fp32 or bf16 (rows may be further apart); tokens int32 [rows] or
+    [rows, n], None for none; workspace: zero-filled uint8 tensor of LOGIT_WORKSPACE_BYTES that the caller keeps, lets
+    few long rows be cut over the device.  Returns a dict: stats [rows, 2] (for the backward pass); logprob in
+    tokens' shape; entropy [rows]; top_ids int32 and top_logprobs [rows, top_k]; those not asked for are left out."""
+    import torch
+    code, rows, vocab, stride = _logit_rows(logits)
+    _require_device(logits, tokens, workspace)
+    dev, f32 = logits.device, torch.float32
+    out = Luts(stats=torch.empty((rows, 2), dtype=f32, device=dev))
+    n, tok, lp, ent, ids, top = 0, None, None, None, None, None
+    if tokens is not None:
+        n = 1 if tokens.dim() == 1 else tokens.shape[-1]
+        tok = _small(tokens, (rows,) if tokens.dim() == 1 else (rows, n), torch.int32, "tokens")
+        out["logprob"] = torch.empty(tokens.shape, dtype=f32, device=dev)
+        lp = out["logprob"].data_ptr()
+    if entropy:
+        out["entropy"] = torch.empty(rows, dtype=f32, device=dev)
+        ent = out["entropy"].data_ptr()
+    if top_k:
+        out["top_ids"] = torch.empty((rows, top_k), dtype=torch.int32, device=dev)
+        out["top_logprobs"] = torch.empty((rows, top_k), dtype=f32, device=dev)
+        ids, top = out["top_ids"].data_ptr(), out["top_logprobs"].data_ptr()
+    ws, ws_bytes = _logit_workspace(workspace)
+    _logit_call("sfb_token_logprobs", lp, ent, out["stats"].data_ptr(), ids, top, logits.data_ptr(), code, tok, rows, vocab,
+                stride, n, top_k, scale, ws, ws_bytes)
+    return out
+
+
+def token_logprobs_backward(logits, tokens, stats, d_logprob=None, entropy=None, d_entropy=None, scale=1.0, out=None):
+    """d_logits of sum d_logprob * logprob + sum d_entropy * entropy (sfb_token_logprobs_backward), from token_logprobs'
+    stats (and entropy, where d_entropy is given); out may be the logits themselves."""
+    import torch
+    code, rows, vocab, stride = _logit_rows(logits)
+    _require_device(logits, tokens, stats, d_logprob, entropy, d_entropy, out)
+    n, f32 = 0, torch.float32
+    tok = grad = None
+    if d_logprob is not None:
+        if tokens is None:
+            raise SfbError(1, "tokens")
+        shape = tuple(tokens.shape) if tokens.dim() != 1 else (rows,)
+        n = 1 if tokens.dim() == 1 else tokens.shape[-1]
+        if tokens.dim() > 2 or shape[0] != rows:
+            raise SfbError(4, "tokens of shape %s" % (tuple(tokens.shape),))
+        tok, grad = _small(tokens, shape, torch.int32, "tokens"), _small(d_logprob, shape, f32, "d_logprob")
+    out = _like_logits(logits, stride, out)
+    _logit_call("sfb_token_logprobs_backward", out.data_ptr(), logits.data_ptr(), code, tok,
+                _small(stats, (rows, 2), f32, "stats"), _small(entropy, (rows,), f32, "entropy"), grad,
+                _small(d_entropy, (rows,), f32, "d_entropy"), rows, vocab, stride, n, scale)
+    return out
+
+
+def _teacher(teacher_ids, teacher_logits, rows):
+    import torch
+    slots = teacher_ids.shape[-1]
+    return (_small(teacher_ids, (rows, slots), torch.int32, "teacher_ids"),
+            _small(teacher_logits, (rows, slots), teacher_logits.dtype, "teacher_logits"), _dtype_code(teacher_logits), slots)
+
+
+def distillation_loss(logits, teacher_ids, teacher_logits, scale=1.0, d_loss=None, out=None, workspace=None):
+    """Divergence of softmax(scale * logits) from a teacher's top logits, per row (sfb_distillation_loss).  teacher_ids
+    int32 and teacher_logits fp32 or bf16 [rows, slots]; ids outside the vocabulary are unused slots.  Returns a dict:
+    row_loss [rows], stats [rows, 2], and with d_loss [rows] (the gradient of each row's loss) also d_logits, written
+    to out (which may be the logits themselves) if given.  workspace as for token_logprobs."""
+    import torch
+    code, rows, vocab, stride = _logit_rows(logits)
+    _require_device(logits, teacher_ids, teacher_logits, d_loss, out, workspace)
+    if out is not None and d_loss is None:
+        raise SfbError(1, "d_loss")
+    ids, z, z_code, slots = _teacher(teacher_ids, teacher_logits, rows)
+    got = Luts(row_loss=torch.empty(rows, dtype=torch.float32, device=logits.device),
+               stats=torch.empty((rows, 2), dtype=torch.float32, device=logits.device))
+    grad = None
+    if d_loss is not None:
+        got["d_logits"] = _like_logits(logits, stride, out)
+        grad = got["d_logits"].data_ptr()
+    ws, ws_bytes = _logit_workspace(workspace)
+    _logit_call("sfb_distillation_loss", got["row_loss"].data_ptr(), got["stats"].data_ptr(), grad, logits.data_ptr(), code,
+                ids, z, z_code, _small(d_loss, (rows,), torch.float32, "d_loss"), rows, vocab, stride, slots, scale, ws,
+                ws_bytes)
+    return got
+
+
+def distillation_loss_backward(logits, teacher_ids, teacher_logits, stats, d_loss, scale=1.0, out=None):
+    """d_logits of sum d_loss * row_loss from distillation_loss's stats (sfb_distillation_loss_backward)."""
+    import torch
+    code, rows, vocab, stride = _logit_rows(logits)
+    _require_device(logits, teacher_ids, teacher_logits, stats, d_loss, out)
+    ids, z, z_code, slots = _teacher(teacher_ids, teacher_logits, rows)
+    out = _like_logits(logits, stride, out)
+    _logit_call("sfb_distillation_loss_backward", out.data_ptr(), logits.data_ptr(), code, ids, z, z_code,
+                _small(stats, (rows, 2), torch.float32, "stats"), _small(d_loss, (rows,), torch.float32, "d_loss"), rows,
+                vocab, stride, slots, scale)
+    return out
+
+
 class LayerWeights(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("wq", "wk", "wv", "wo", "w1", "w2", "bq", "bk", "bv", "bo", "b1", "b2",
                                           "ln1_g", "ln1_b", "ln2_g", "ln2_b", "wqkv", "bqkv")]
@@ -1058,3 +1230,13 @@ class Model:
             C.c_uint32(B), C.c_uint32(L // self.bs), C.c_uint32(self.heads), C.c_uint32(self.d), C.c_uint32(self.ffn),
             C.c_uint32(vocab), _dev(ws), C.c_size_t(ws.numel())), "sfb_model_forward")
         return out
+
+    def score(self, ids, tokens=None, top_k=0, scale=1.0, entropy=False, mask=None, valid_len=None, workspace=None):
+        """The model's answer at every position of ids [B, L]: token_logprobs() of its logits (a dict; rows are the
+        B * L positions in order).  tokens int32 [B, L] or [B, L, n]: the tokens whose log probabilities are asked."""
+        logits = self.forward(ids, mask=mask, valid_len=valid_len, want_logits=True)["logits"]
+        if tokens is not None:
+            if tokens.dim() not in (2, 3) or tuple(tokens.shape[:2]) != tuple(ids.shape):
+                raise SfbError(4, "tokens of shape %s" % (tuple(tokens.shape),))
+            tokens = tokens.reshape((ids.numel(),) + tuple(tokens.shape[2:]))
+        return token_logprobs(logits, tokens, top_k, scale, entropy, workspace)

@@ -36,7 +36,7 @@ LIB = os.path.join(BUILD, "libsfbert_emu.so")
 CLANG = "/opt/rocm/lib/llvm/bin/clang++"
 
 KERNEL_SOURCES = ["fused_attention.hip", "fused_backward.hip", "unfused_attention.hip", "layer_ops.hip", "runtime.hip",
-                  "encoder_layer.hip"]
+                  "encoder_layer.hip", "logit_ops.hip"]
 HOST_SOURCES = ["descriptors.cpp"]
 HEADERS = ["common.hip.h", "tiles.hip.h", "tile_index.h"]
 
@@ -461,6 +461,7 @@ def load(tag="", defines=()):
         else:
             os.environ["SFBERT_HIP_LIB"] = saved
     mod._stream = lambda: None
+    mod._require_device = lambda *tensors: None
     mod.to_device = lambda a: tensor(np.ascontiguousarray(a).view(np.uint8).reshape(-1))
     lib = mod.lib
     lib.emu_guarded_alloc.restype = C.c_void_p
