@@ -22,6 +22,8 @@ constexpr float kWide = 1.0e29f;
 template <typename T> struct LogitVec;
 template <> struct LogitVec<float> {
     static constexpr int N = 4;
+    static constexpr uint32_t kMasked = 0xff800000u;   // -inf
+    static constexpr uint32_t kMaskedOne = kMasked;
     __device__ static __forceinline__ void unpack(u32x4 raw, float (&v)[N]) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
@@ -35,11 +37,16 @@ template <> struct LogitVec<float> {
         for (int i = 0; i < N; ++i) r[i] = __builtin_bit_cast(uint32_t, v[i]);
         return r;
     }
+    // one logit's bits and their value (apart, so that a load need not be waited for where it is issued)
+    __device__ static __forceinline__ uint32_t bits(const float* p) { return *(const uint32_t*)p; }
+    __device__ static __forceinline__ float value(uint32_t b) { return __builtin_bit_cast(float, b); }
     __device__ static __forceinline__ float load(const float* p) { return *p; }
     __device__ static __forceinline__ void store(float* p, float v) { *p = v; }
 };
 template <> struct LogitVec<__bf16> {
     static constexpr int N = 8;
+    static constexpr uint32_t kMasked = 0xff80ff80u;   // -inf, twice
+    static constexpr uint32_t kMaskedOne = 0xff80u;
     __device__ static __forceinline__ void unpack(u32x4 raw, float (&v)[N]) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -53,6 +60,8 @@ template <> struct LogitVec<__bf16> {
         for (int i = 0; i < 4; ++i) r[i] = pack_bf16(v[2 * i], v[2 * i + 1]);
         return r;
     }
+    __device__ static __forceinline__ uint32_t bits(const __bf16* p) { return *(const uint16_t*)p; }
+    __device__ static __forceinline__ float value(uint32_t b) { return bf16_bits_to_f32(b); }
     __device__ static __forceinline__ float load(const __bf16* p) { return bf16_bits_to_f32(*(const uint16_t*)p); }
     __device__ static __forceinline__ void store(__bf16* p, float v) { *(uint16_t*)p = (uint16_t)pack_bf16(v, 0.f); }
 };
@@ -69,98 +78,358 @@ template <typename T> struct RowSpan {
         vecs = (vocab - head) / N;
         tail = vocab - head - vecs * N;
     }
+    // the same division of another row with the same alignment
+    __device__ __forceinline__ RowSpan onto(const T* r) const {
+        RowSpan s(*this);
+        s.row = r;
+        return s;
+    }
     // element index of the edge element thread t takes care of (one each), or -1
     __device__ __forceinline__ int32_t edge(uint32_t t) const {
         if (t < head) return (int32_t)t;
         if (t < head + tail) return (int32_t)(head + vecs * LogitVec<T>::N + (t - head));
         return -1;
     }
-    __device__ __forceinline__ u32x4 vec(uint32_t i) const { return *(const u32x4*)(row + head + (size_t)i * LogitVec<T>::N); }
+    // vector `base + i`, base the same for the whole wave: its address stays in scalar registers
+    __device__ __forceinline__ const u32x4* at(uint32_t base, uint32_t i) const {
+        return (const u32x4*)((const char*)(row + head) + (size_t)base * 16 + i * 16);
+    }
     __device__ __forceinline__ uint32_t index(uint32_t i) const { return head + i * LogitVec<T>::N; }
 };
 
-// What a lane knows of its part of a row: sum and dot are relative to the scaled reference ref2, which lags the
-// running maximum by at most kLazyRescaleLog2 powers of two, so that it hardly ever moves after the first vector.
-struct RowSum {
-    float ref, ref2;   // reference logit and fl(ref c)
-    float top;         // largest logit (NaN left out)
-    float sum, dot;    // sum 2^t, sum 2^t t with t = x c - ref2
-    __device__ __forceinline__ void clear() { ref = top = -kInf; ref2 = kNoReference; sum = dot = 0.f; }
-
-    // 2^t t with t = -inf standing for 0 (a masked logit); a NaN reaches both sums through 2^t
-    template <bool ENTROPY, int N>
-    __device__ __forceinline__ void add(const float (&v)[N], float c) {
-        float hi = v[0];
-#pragma unroll
-        for (int i = 1; i < N; ++i) hi = fmaxf(hi, v[i]);
-        top = fmaxf(top, hi);
-        const float hi2 = hi * c;
-        if (hi2 > ref2 + kLazyRescaleLog2) {
-            const float d = ref2 - hi2, f = exp2_fast(d);
-            if (ENTROPY) dot = f * (dot + fmaxf(d, -256.f) * sum);
-            sum *= f;
-            ref = hi;
-            ref2 = hi2;
-        }
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float t = fmaf(v[i], c, -ref2), e = exp2_fast(t);
-            sum += e;
-            if (ENTROPY) dot = fmaf(e, fmaxf(t, -256.f), dot);
-        }
-    }
-    // the same relative to a given reference, subtracted before scaling
-    template <bool ENTROPY, int N>
-    __device__ __forceinline__ void add_wide(const float (&v)[N], float c, float m) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float t = (v[i] - m) * c, e = exp2_fast(t);
-            sum += e;
-            if (ENTROPY) dot = fmaf(e, fmaxf(t, -256.f), dot);
-        }
-    }
-    // from relative to fl(ref c) to relative to ref c: the reference of different lanes, and of the backward pass, is
-    // the logit itself
-    template <bool ENTROPY> __device__ __forceinline__ void settle(float c) {
-        if (ref == -kInf) return;
-        const float d = fmaf(ref, c, -ref2), f = exp2_fast(-d);
-        if (ENTROPY) dot = f * (dot - d * sum);
-        sum *= f;
-    }
-    // to a reference m >= ref
-    template <bool ENTROPY> __device__ __forceinline__ void move(float m, float c) {
-        const float d = ref == m ? 0.f : (ref - m) * c, f = exp2_fast(d);
-        if (ENTROPY) dot = f * (dot + fmaxf(d, -256.f) * sum);
-        sum *= f;
-        ref = m;
-    }
+// The part of a row one work-group takes: vectors [v0, v1) and elements [e0, e1), which add the row's first elements to
+// the first part and its last ones to the last.
+struct Slice {
+    uint32_t v0, v1, e0, e1;
+    int32_t edge;   // the edge element of this thread, or -1
 };
+template <typename T>
+__device__ __forceinline__ Slice slice_of(const RowSpan<T>& span, uint32_t vocab, uint32_t part, uint32_t parts, uint32_t each,
+                                          uint32_t t) {
+    Slice s;
+    s.v0 = part * each < span.vecs ? part * each : span.vecs;
+    s.v1 = part + 1 == parts || s.v0 + each > span.vecs ? span.vecs : s.v0 + each;
+    s.e0 = part == 0 ? 0 : span.index(s.v0);
+    s.e1 = part + 1 == parts ? vocab : span.index(s.v1);
+    s.edge = span.edge(t);
+    if (s.edge >= 0 && ((uint32_t)s.edge < s.e0 || (uint32_t)s.edge >= s.e1)) s.edge = -1;
+    return s;
+}
 
-template <int THREADS> __device__ __forceinline__ float group_max(float v, float* red) {
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
+// ---- reductions -----------------------------------------------------------------------------------------------
+template <int CTRL> __device__ __forceinline__ float dpp(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float lane(float v, int i) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i));
+}
+// Within 16 lanes by DPP moves (neighbours, pairs, mirrored halves), the four results by lane reads: no LDS round trips.
+// All lanes get the same bits.
+__device__ __forceinline__ float wave_max(float v) {
+    v = fmaxf(v, dpp<0xB1>(v));
+    v = fmaxf(v, dpp<0x4E>(v));
+    v = fmaxf(v, dpp<0x141>(v));
+    v = fmaxf(v, dpp<0x140>(v));
+    return fmaxf(fmaxf(lane(v, 0), lane(v, 16)), fmaxf(lane(v, 32), lane(v, 48)));
+}
+__device__ __forceinline__ float wave_sum(float v) {
+    v += dpp<0xB1>(v);
+    v += dpp<0x4E>(v);
+    v += dpp<0x141>(v);
+    v += dpp<0x140>(v);
+    return (lane(v, 0) + lane(v, 16)) + (lane(v, 32) + lane(v, 48));
+}
+// red: THREADS / 64 floats for max, twice that for sums.  Sums are taken in an order that depends on THREADS alone.
+// publish() is called between the two barriers, by every thread.
+template <int THREADS, typename P> __device__ __forceinline__ float group_max(float v, float* red, P publish) {
+    v = wave_max(v);
+    __syncthreads();
+    if (THREADS > 64 && (threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    publish();
+    __syncthreads();
     if (THREADS == 64) return v;
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
     v = red[0];
 #pragma unroll
     for (int w = 1; w < THREADS / 64; ++w) v = fmaxf(v, red[w]);
     return v;
 }
-// sums in an order that depends on nothing but THREADS
-template <int THREADS> __device__ __forceinline__ float group_sum(float v, float* red) {
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d);
-    if (THREADS == 64) return v;
+template <int THREADS, bool BOTH> __device__ __forceinline__ void group_sum(float& a, float& b, float* red) {
+    a = wave_sum(a);
+    if (BOTH) b = wave_sum(b);
+    if (THREADS == 64) return;
+    constexpr int W = THREADS / 64;
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) {
+        red[threadIdx.x >> 6] = a;
+        if (BOTH) red[W + (threadIdx.x >> 6)] = b;
+    }
     __syncthreads();
-    v = red[0];
+    a = red[0];
+    if (BOTH) b = red[W];
 #pragma unroll
-    for (int w = 1; w < THREADS / 64; ++w) v += red[w];
-    return v;
+    for (int w = 1; w < W; ++w) {
+        a += red[w];
+        if (BOTH) b += red[W + w];
+    }
 }
+
+// ---- the softmax sums of a row --------------------------------------------------------------------------------
+struct RowSum {
+    float m;           // reference logit (-inf: nothing but -inf and NaN)
+    float sum, dot;    // sum 2^t, sum 2^t t with t = (x - m) c
+    float top;         // this thread's largest logit (NaN left out)
+};
+
+template <int N> __device__ __forceinline__ float largest(const float (&x)[N]) {
+    float hi = x[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) hi = fmaxf(hi, x[i]);
+    return hi;
+}
+template <typename T, int G> __device__ __forceinline__ float largest_of(const u32x4* raw) {
+    float hi = -kInf;
+#pragma unroll
+    for (int u = 0; u < G; ++u) {
+        float x[LogitVec<T>::N];
+        LogitVec<T>::unpack(raw[u], x);
+        hi = fmaxf(hi, largest(x));
+    }
+    return hi;
+}
+
+// 2^t and 2^t t; t = -inf (a masked logit) stands for 0 in both, a NaN reaches both.
+template <bool ENTROPY, bool CLAMP = true> __device__ __forceinline__ void add_term(float t, float& sum, float& dot) {
+    const float e = exp2_fast(t);
+    sum += e;
+    if (ENTROPY) dot = fmaf(e, CLAMP ? fmaxf(t, -256.f) : t, dot);
+}
+// The terms of G vectors relative to ref2.  Clamping t costs a seventh of the entropy's instructions and is for masked
+// logits alone, so it is left out until a 0 * -inf shows that there are some: that step is then done again, and the
+// wave clamps from there on.
+template <typename T, int G, bool ENTROPY>
+__device__ __forceinline__ void add_terms(const u32x4* raw, float c, float ref2, float& sum, float& dot, bool& clamp) {
+    constexpr int N = LogitVec<T>::N;
+    const float sum0 = sum, dot0 = dot;
+    if (!ENTROPY || !clamp) {
+#pragma unroll
+        for (int u = 0; u < G; ++u) {
+            float x[N];
+            LogitVec<T>::unpack(raw[u], x);
+#pragma unroll
+            for (int i = 0; i < N; ++i) add_term<ENTROPY, false>(fmaf(x[i], c, -ref2), sum, dot);
+        }
+        if (!ENTROPY || __builtin_amdgcn_ballot_w64(dot != dot) == 0) return;
+        clamp = true;
+        sum = sum0;
+        dot = dot0;
+    }
+#pragma unroll
+    for (int u = 0; u < G; ++u) {
+        u32x4 again = raw[u];
+        asm volatile("" : "+v"(again));   // (nothing of the first attempt is kept in registers for this one)
+        float x[N];
+        LogitVec<T>::unpack(again, x);
+#pragma unroll
+        for (int i = 0; i < N; ++i) add_term<ENTROPY, true>(fmaf(x[i], c, -ref2), sum, dot);
+    }
+}
+
+// Logits whose scaled values pass this in either direction are subtracted from the maximum before they are scaled.
+__device__ __forceinline__ bool is_wide(float m, float c) { return fabsf(m * c) > kWide && fabsf(m) < kInf; }
+
+template <int V> struct Int { static constexpr int value = V; };
+
+// G vectors of every thread, `base` the first thread's first vector, THREADS apart.  The loads are unconditional (past
+// the end: the last vector), so that all of them are in flight at once.  Logits are read once: nontemporal loads.
+template <typename T, int THREADS, int G>
+__device__ __forceinline__ void load_vectors(const RowSpan<T>& span, const Slice& s, uint32_t base, uint32_t t, u32x4* raw) {
+#pragma unroll
+    for (int u = 0; u < G; ++u) {
+        const uint32_t b = base + u * THREADS < s.v1 ? base + u * THREADS : s.v1 - 1, last = s.v1 - 1 - b;
+        raw[u] = __builtin_nontemporal_load(span.at(b, t < last ? t : last));
+    }
+}
+// f(count, vectors, base) for these G vectors: all at once where the work-group has all of them, else one by one as far
+// as the slice goes.  MASK: what lies past its end is first overwritten with -inf, which counts nowhere.
+template <typename T, int THREADS, int G, bool MASK, typename F>
+__device__ __forceinline__ void step_vectors(const Slice& s, uint32_t base, uint32_t t, u32x4* raw, F f) {
+    if (base + G * THREADS <= s.v1) {
+        f(Int<G>(), raw, base);
+        return;
+    }
+#pragma unroll
+    for (int u = 0; u < G; ++u) {
+        const uint32_t b = base + u * THREADS;
+        if (b < s.v1) {
+            if (MASK && b + t >= s.v1) raw[u] = u32x4{LogitVec<T>::kMasked, LogitVec<T>::kMasked, LogitVec<T>::kMasked, LogitVec<T>::kMasked};
+            f(Int<1>(), raw + u, b);
+        }
+    }
+}
+
+// A slice held in registers: NV vectors per thread, read before anything is computed, so that the maximum is known when
+// the exponentials begin.
+template <typename T, int THREADS, int NV> struct Held {
+    static constexpr int N = LogitVec<T>::N;
+    static constexpr int G = NV < 2 ? NV : 2;   // vectors per step
+    u32x4 raw[NV];
+    uint32_t edge;   // bits of the edge element
+    __device__ __forceinline__ void load(const RowSpan<T>& span, const Slice& s, uint32_t t) {
+        edge = LogitVec<T>::kMaskedOne;
+        if (s.edge >= 0) edge = LogitVec<T>::bits(span.row + s.edge);
+        if (s.v1 > s.v0) load_vectors<T, THREADS, NV>(span, s, s.v0, t, raw);
+    }
+    // f(x, base, vector) for every vector of this thread, which is the t-th from base
+    template <typename F> __device__ __forceinline__ void each(const Slice& s, uint32_t t, F f) const {
+#pragma unroll
+        for (int u = 0; u < NV; ++u) {
+            const uint32_t base = s.v0 + u * THREADS;
+            if (base + t < s.v1) {
+                float x[N];
+                LogitVec<T>::unpack(raw[u], x);
+                f(x, base);
+            }
+        }
+    }
+    template <bool MASK, typename F> __device__ __forceinline__ void steps(const Slice& s, uint32_t t, F f) {
+#pragma unroll
+        for (int g = 0; g < NV; g += G)
+            if (s.v0 + g * THREADS < s.v1) step_vectors<T, THREADS, G, MASK>(s, s.v0 + g * THREADS, t, raw + g, f);
+    }
+    // publish(largest logit) is called by every thread before the work-group meets for the maximum, met() right after
+    // (what it leaves in shared memory can be read when the sums are there).
+    template <bool ENTROPY, typename P, typename M>
+    __device__ __forceinline__ RowSum sums(const Slice& s, uint32_t t, float c, float* red, P publish, M met) {
+        RowSum r;
+        const float single = LogitVec<T>::value(edge);
+        r.top = single;
+        steps<true>(s, t, [&](auto count, const u32x4* x, uint32_t) { r.top = fmaxf(r.top, largest_of<T, decltype(count)::value>(x)); });
+        r.m = group_max<THREADS>(r.top, red, [&]() { publish(r.top); });
+        met();
+        r.sum = r.dot = 0.f;
+        const float m = r.m == -kInf ? 0.f : r.m;
+        if (!is_wide(m, c)) {
+            const float mc = m * c, d = fmaf(m, c, -mc);   // d: what rounding left out of m c
+            bool clamp = false;
+            steps<false>(s, t, [&](auto count, const u32x4* x, uint32_t) {
+                add_terms<T, decltype(count)::value, ENTROPY>(x, c, mc, r.sum, r.dot, clamp);
+            });
+            add_term<ENTROPY>(fmaf(single, c, -mc), r.sum, r.dot);
+            const float f = exp2_fast(-d);
+            if (ENTROPY) r.dot = f * (r.dot - d * r.sum);
+            r.sum *= f;
+        } else {
+            each(s, t, [&](const float (&x)[N], uint32_t) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) add_term<ENTROPY>((x[i] - m) * c, r.sum, r.dot);
+            });
+            add_term<ENTROPY>((single - m) * c, r.sum, r.dot);
+        }
+        group_sum<THREADS, ENTROPY>(r.sum, r.dot, red);
+        return r;
+    }
+};
+
+// A row longer than the registers of its work-group, in one pass.  Each thread keeps its sums relative to a reference of
+// its own that lags its largest logit by at most kLazyRescaleLog2 powers of two, so that it hardly ever moves after the
+// first step.
+template <typename T, int THREADS> struct Streamed {
+    static constexpr int N = LogitVec<T>::N;
+    static constexpr int G = 4, P = 2;   // vectors in flight, and per step
+
+    // f(x, base) for every vector of this thread, as above
+    template <typename F> static __device__ __forceinline__ void each(const RowSpan<T>& span, const Slice& s, uint32_t t, F f) {
+        for (uint32_t base = s.v0; base < s.v1; base += THREADS * G) {
+            u32x4 raw[G];
+            load_vectors<T, THREADS, G>(span, s, base, t, raw);
+#pragma unroll
+            for (int u = 0; u < G; ++u)
+                if (base + u * THREADS + t < s.v1) {
+                    float x[N];
+                    LogitVec<T>::unpack(raw[u], x);
+                    f(x, base + u * THREADS);
+                }
+        }
+    }
+    // early(f) is called once, by every thread, f() giving its largest logit among the first vectors; meet(count, vectors,
+    // largest, base) for what every step holds.
+    template <bool ENTROPY, typename E, typename M>
+    static __device__ __forceinline__ RowSum sums(const RowSpan<T>& span, const Slice& s, uint32_t t, float c, float* red, E early, M meet) {
+        RowSum r;
+        r.top = -kInf;
+        r.sum = r.dot = 0.f;
+        float ref = -kInf, ref2 = kNoReference;   // the reference logit and fl(ref c)
+        bool clamp = false;
+        auto raise = [&](float hi) {
+            r.top = fmaxf(r.top, hi);
+            const float hi2 = hi * c;
+            const bool higher = hi2 > ref2 + kLazyRescaleLog2;
+            if (__builtin_amdgcn_ballot_w64(higher) != 0) {   // (a branch of the whole wave, hardly ever taken)
+                asm volatile("" : : : "memory");   // (kept a branch: made a select, it would cost every step)
+                if (higher) {
+                    const float d = ref2 - hi2, f = exp2_fast(d);
+                    if (ENTROPY) r.dot = f * (r.dot + fmaxf(d, -256.f) * r.sum);
+                    r.sum *= f;
+                    ref = hi;
+                    ref2 = hi2;
+                }
+            }
+        };
+        uint32_t edge = LogitVec<T>::kMaskedOne;
+        if (s.edge >= 0) edge = LogitVec<T>::bits(span.row + s.edge);
+        auto step = [&](auto count, const u32x4* raw, uint32_t base) {
+            const float hi = largest_of<T, decltype(count)::value>(raw);
+            raise(hi);
+            meet(count, raw, hi, base);
+            add_terms<T, decltype(count)::value, ENTROPY>(raw, c, ref2, r.sum, r.dot, clamp);
+        };
+        auto steps = [&](u32x4* raw, uint32_t base) {
+#pragma unroll
+            for (int g = 0; g < G; g += P)
+                if (base + g * THREADS < s.v1) step_vectors<T, THREADS, P, true>(s, base + g * THREADS, t, raw + g, step);
+        };
+        if (s.v1 > s.v0) {   // (the second vectors are on their way while early() has the work-group meet)
+            u32x4 raw[2 * G];
+            load_vectors<T, THREADS, 2 * G>(span, s, s.v0, t, raw);
+            early([&]() {
+                float hi = LogitVec<T>::value(edge);
+                step_vectors<T, THREADS, G, true>(s, s.v0, t, raw, [&](auto count, const u32x4* x, uint32_t) {
+                    hi = fmaxf(hi, largest_of<T, decltype(count)::value>(x));
+                });
+                return hi;
+            });
+            steps(raw, s.v0);
+            if (s.v0 + G * THREADS < s.v1) steps(raw + G, s.v0 + G * THREADS);
+        } else {
+            early([&]() { return LogitVec<T>::value(edge); });
+        }
+        for (uint32_t base = s.v0 + 2 * THREADS * G; base < s.v1; base += THREADS * G) {
+            u32x4 raw[G];
+            load_vectors<T, THREADS, G>(span, s, base, t, raw);
+            steps(raw, base);
+        }
+        const float single = LogitVec<T>::value(edge);
+        raise(single);
+        add_term<ENTROPY>(fmaf(single, c, -ref2), r.sum, r.dot);
+        const float top = group_max<THREADS>(r.top, red, []() {});
+        if (is_wide(top, c)) {
+            r.sum = r.dot = 0.f;
+            each(span, s, t, [&](const float (&x)[N], uint32_t) {
+#pragma unroll
+                for (int i = 0; i < N; ++i) add_term<ENTROPY>((x[i] - top) * c, r.sum, r.dot);
+            });
+            if (s.edge >= 0) add_term<ENTROPY>((single - top) * c, r.sum, r.dot);
+        } else if (ref != -kInf) {   // from the thread's fl(ref c) to the row's largest logit
+            const float rounding = fmaf(ref, c, -ref2);
+            const float d = ref == top ? -rounding : (ref - top) * c - rounding, f = exp2_fast(d);
+            if (ENTROPY) r.dot = f * (r.dot + fmaxf(d, -256.f) * r.sum);
+            r.sum *= f;
+        }
+        r.m = top;
+        group_sum<THREADS, ENTROPY>(r.sum, r.dot, red);
+        return r;
+    }
+};
 
 // Order of the alternatives as whole numbers: larger logits first, -0 as +0, NaN above everything; 0 is below every
 // logit.  A composite's low word is the complement of the index: of equal logits the lowest index comes first.
@@ -174,147 +443,242 @@ __device__ __forceinline__ float logit_of(uint32_t order) {
 }
 __device__ __forceinline__ uint64_t composite(uint32_t order, uint32_t index) { return ((uint64_t)order << 32) | (uint32_t)~index; }
 
-// The k largest of a row whose threads know the largest logit each of them has met.  The k-th largest of those is at
-// most the row's k-th largest logit, and about k logits reach it (with 256 threads and k = 20: about 21), so the row
-// itself is only read again where a thread's largest does: a handful of vectors.  Rows with more equal or clustered
-// logits than the list holds take the exact threshold from counts over the whole row instead.
+// The k largest of a slice whose threads know the largest logit each of them has met.  The largest logits of 64 or 256
+// groups of threads are compared: the k-th largest of those is at most the slice's k-th largest logit, and hardly more
+// than k logits reach it (256 groups and k = 20: 21 expected), so only the threads whose own largest does look at their
+// vectors again.  A slice with more equal or clustered logits than the list holds takes the exact threshold instead.
 template <typename T, int THREADS> struct TopSelect {
     static constexpr int LIST = 512;
     static constexpr int N = LogitVec<T>::N;
-    uint64_t* list;       // [LIST] in shared memory
-    uint32_t* words;      // [THREADS] in shared memory
-    uint32_t* count;      // in shared memory
-
-    __device__ __forceinline__ void append(uint32_t order, uint32_t index) {
-        const uint32_t at = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-        if (at < (uint32_t)LIST) list[at] = composite(order, index);
+    static constexpr int GROUPS = THREADS < 256 ? THREADS : 256;
+    static constexpr int LOW_BIT = sizeof(T) == 2 ? 16 : 0;   // bf16 logits are told apart by the upper half
+    static constexpr int VECTORS = 256;
+    struct Shared {
+        u32x4 vectors[VECTORS];       // vectors that hold a logit above the threshold
+        uint64_t list[LIST];          // composites
+        uint32_t at[VECTORS];         // index of each vector's first element
+        uint32_t words[GROUPS + 2];   // the groups' largest logits, and what came of them
+        uint32_t count, n_vectors;
+    };
+    static __device__ __forceinline__ Shared& shared() {
+        __shared__ Shared memory;
+        return memory;
     }
 
-    // the largest threshold reached by at least k of the threads' largest logits; *exact: it is one of them
-    __device__ uint32_t threshold(uint32_t mine, uint32_t k, bool* exact) {
-        const uint32_t t = threadIdx.x, lane = t & 63;
+    static __device__ __forceinline__ void append(uint32_t order, uint32_t index) {
+        const uint32_t at = __hip_atomic_fetch_add(&shared().count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        if (at < (uint32_t)LIST) shared().list[at] = composite(order, index);
+    }
+    static __device__ __forceinline__ void clear_count() {
         __syncthreads();
-        words[t] = mine;
+        if (threadIdx.x == 0) shared().count = 0;
         __syncthreads();
-        uint32_t own[THREADS / 64];
+    }
+
+    // The largest value that at least k of 64 * W groups' largest logits reach, found bit by bit by one wave; it ends
+    // early where exactly k reach it (*all: it did not, the threshold is one of them).
+    template <int W> static __device__ __forceinline__ uint32_t search(uint32_t k, uint32_t* all) {
+        uint32_t own[W], limit = 0;
 #pragma unroll
-        for (int i = 0; i < THREADS / 64; ++i) own[i] = words[i * 64 + lane];
-        uint32_t limit = 0;
-        bool all = true;
-        for (int bit = 31; bit >= 0; --bit) {   // every wave does the same
+        for (int i = 0; i < W; ++i) own[i] = shared().words[i * 64 + (threadIdx.x & 63)];
+        *all = 1;
+        for (int bit = 31; bit >= LOW_BIT; --bit) {
             const uint32_t next = limit | (1u << bit);
             uint32_t n = 0;
 #pragma unroll
-            for (int i = 0; i < THREADS / 64; ++i) n += (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(own[i] >= next));
+            for (int i = 0; i < W; ++i) n += (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(own[i] >= next));
             if (n >= k) limit = next;
-            if (n == k) { all = false; break; }
+            if (n == k) { *all = 0; break; }
         }
-        *exact = all;
+        // (orders of negative bf16 logits end in ones)
+        if (LOW_BIT && !(limit >> 31)) limit |= (1u << LOW_BIT) - 1;
         return limit;
     }
-
-    // appends the row's logits above (strict) or from `limit` on, reading only where a thread's largest reaches it
-    __device__ void collect(const RowSpan<T>& span, uint32_t v0, uint32_t v1, int32_t edge, uint32_t mine, uint32_t limit,
-                            bool strict) {
+    // A threshold that at least k logits of the threads' largest reach, in three parts with a barrier after the first and
+    // the second: every thread publishes its largest logit (and count is cleared), one wave searches, all read the
+    // result; *exact: it is one of those logits.  Up to k = 32 the threads form 64 groups (k = 20: 24 logits expected
+    // above the threshold), beyond that up to 256.
+    static __device__ __forceinline__ void publish(float top, bool any, uint32_t k) {
         const uint32_t t = threadIdx.x;
-        __shared__ uint32_t n_threads;
+        uint32_t mine = any ? order_of(top) : 0u;
+        const bool wide = THREADS > 64 && k > 32;
+        if (THREADS >= 128) mine = pair_max<0xB1>(mine, THREADS >= 512 || !wide);
+        if (THREADS >= 256) mine = pair_max<0x4E>(mine, THREADS >= 1024 || !wide);
+        if (THREADS >= 512 && !wide) mine = pair_max<0x141>(mine, true);
+        if (THREADS >= 1024 && !wide) mine = pair_max<0x140>(mine, true);
+        const uint32_t per = wide ? THREADS / GROUPS : THREADS / 64;
+        if (t % per == 0) shared().words[t / per] = mine;
+        if (t == 0) shared().count = shared().n_vectors = 0;
+    }
+    static __device__ __forceinline__ void find(uint32_t k) {
+        if (threadIdx.x >= 64) return;
+        uint32_t all;
+        const uint32_t limit = THREADS > 64 && k > 32 ? search<GROUPS / 64>(k, &all) : search<1>(k, &all);
+        if (threadIdx.x == 0) { shared().words[GROUPS] = limit; shared().words[GROUPS + 1] = all; }
+    }
+    static __device__ __forceinline__ uint32_t found(bool* exact) {
+        *exact = shared().words[GROUPS + 1] != 0;
+        return shared().words[GROUPS];
+    }
+    static __device__ __forceinline__ uint32_t threshold(float top, bool any, uint32_t k, bool* exact) {
         __syncthreads();
-        if (t == 0) { *count = 0; n_threads = 0; }
+        publish(top, any, k);
         __syncthreads();
-        const bool reached = strict ? mine > limit : mine >= limit;
-        if (reached) words[__hip_atomic_fetch_add(&n_threads, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP)] = t;
+        find(k);
         __syncthreads();
-        const uint32_t each = (v1 - v0 + THREADS - 1) / THREADS, work = n_threads * each;
-        for (uint32_t i = t; i < work; i += THREADS) {
-            const uint32_t v = v0 + words[i / each] + (i % each) * THREADS;
-            if (v < v1) {
-                float x[N];
-                LogitVec<T>::unpack(span.vec(v), x);
-#pragma unroll
-                for (int u = 0; u < N; ++u) {
-                    const uint32_t o = order_of(x[u]);
-                    if (strict ? o > limit : o >= limit) append(o, span.index(v) + u);
-                }
-            }
-            if (*(volatile uint32_t*)count > (uint32_t)LIST) break;
-        }
-        if (reached && edge >= 0) {
-            const uint32_t o = order_of(LogitVec<T>::load(span.row + edge));
-            if (strict ? o > limit : o >= limit) append(o, (uint32_t)edge);
-        }
-        __syncthreads();
+        return found(exact);
+    }
+    template <int CTRL> static __device__ __forceinline__ uint32_t pair_max(uint32_t v, bool take) {
+        const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+        return take && o > v ? o : v;
     }
 
-    // logits of the row that reach `limit`
-    __device__ uint32_t reaching(const RowSpan<T>& span, uint32_t v0, uint32_t v1, int32_t edge, uint32_t limit) {
+    // appends the logits of one vector that reach `least`
+    static __device__ __forceinline__ void scan(const float (&x)[N], uint32_t index, float least) {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (x[i] >= least) append(order_of(x[i]), index + i);
+    }
+
+    // What follows reads the slice again, element by element in groups of consecutive ones.
+    template <typename F> static __device__ __forceinline__ void elements(const RowSpan<T>& span, const Slice& s, F f) {
+        for (uint32_t j0 = s.e0; j0 < s.e1; j0 += THREADS) {
+            const uint32_t j = j0 + threadIdx.x;
+            if (!f(j < s.e1 ? order_of(LogitVec<T>::load(span.row + j)) : 0u, j)) break;
+        }
+    }
+    static __device__ uint32_t reaching(const RowSpan<T>& span, const Slice& s, uint32_t limit) {
         uint32_t n = 0;
-        for (uint32_t v = v0 + threadIdx.x; v < v1; v += THREADS) {
-            float x[N];
-            LogitVec<T>::unpack(span.vec(v), x);
-#pragma unroll
-            for (int u = 0; u < N; ++u) n += order_of(x[u]) >= limit;
-        }
-        if (edge >= 0) n += order_of(LogitVec<T>::load(span.row + edge)) >= limit;
+        elements(span, s, [&](uint32_t order, uint32_t) { n += order >= limit; return true; });
+        clear_count();
+        if (n) __hip_atomic_fetch_add(&shared().count, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
         __syncthreads();
-        if (threadIdx.x == 0) *count = 0;
-        __syncthreads();
-        if (n) __hip_atomic_fetch_add(count, n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-        __syncthreads();
-        return *count;
+        return shared().count;
     }
-
-    // appends the `want` lowest-index logits equal to `limit`: groups of consecutive elements in rising order, until
-    // there are enough
-    __device__ void collect_equal(const RowSpan<T>& span, uint32_t vocab, uint32_t limit, uint32_t want) {
-        const uint32_t t = threadIdx.x, lane = t & 63;
-        uint32_t have = 0;
-        for (uint32_t j0 = 0; j0 < vocab && have < want; j0 += THREADS) {
-            const uint32_t j = j0 + t;
-            const bool equal = j < vocab && order_of(LogitVec<T>::load(span.row + j)) == limit;
-            const uint64_t in_wave = __builtin_amdgcn_ballot_w64(equal);
+    // the exact k largest: those above the k-th largest value, and of those equal to it the lowest-index ones
+    static __device__ void select_exactly(const RowSpan<T>& span, const Slice& s, uint32_t k, uint32_t limit, bool known) {
+        if (s.e1 - s.e0 <= k) {
+            clear_count();
+            elements(span, s, [&](uint32_t order, uint32_t j) {
+                if (j < s.e1) append(order, j);
+                return true;
+            });
             __syncthreads();
-            if (lane == 0) words[t >> 6] = (uint32_t)__builtin_popcountll(in_wave);
-            __syncthreads();
-            uint32_t at = have + (uint32_t)__builtin_popcountll(in_wave & ((1ull << lane) - 1));
-            for (uint32_t w = 0; w < THREADS / 64; ++w) {
-                if (w < (t >> 6)) at += words[w];
-                have += words[w];
-            }
-            if (equal && at < want) list[*count + at] = composite(limit, j);
+            return;
         }
-        __syncthreads();
-        if (t == 0) *count += want;
-        __syncthreads();
-    }
-
-    // leaves at least the k largest of the row, as composites, in list[0 .. *count).  top: the thread's largest logit,
-    // any: it has one; nan: the row holds NaN (which the threads' largest leave out)
-    __device__ void select(const RowSpan<T>& span, uint32_t vocab, int32_t edge, float top, bool any, bool nan, uint32_t k) {
-        const uint32_t v0 = 0, v1 = span.vecs;
-        const uint32_t mine = nan ? 0xffffffffu : any ? order_of(top) : 0u;
-        bool few = false;
-        uint32_t limit = 0;
-        if (!nan) {
-            bool exact;
-            limit = threshold(mine, k, &exact);
-            collect(span, v0, v1, edge, mine, limit, false);
-            if (*count <= (uint32_t)LIST) return;
-            if (exact) {   // mostly one value (a masked vocabulary): the k-th largest if fewer than k are above it
-                collect(span, v0, v1, edge, mine, limit, true);
-                few = *count < k;
-            }
-        }
-        if (!few) {
+        // (limit given: the k-th largest if fewer than k logits are above it -- a masked vocabulary)
+        if (!known || reaching(span, s, limit + 1) >= k) {
             limit = 0;
             for (int bit = 31; bit >= 0; --bit) {
                 const uint32_t next = limit | (1u << bit);
-                if (reaching(span, v0, v1, edge, next) >= k) limit = next;
+                if (reaching(span, s, next) >= k) limit = next;
             }
-            collect(span, v0, v1, edge, mine, limit, true);
         }
-        collect_equal(span, vocab, limit, k - *count);
+        clear_count();
+        elements(span, s, [&](uint32_t order, uint32_t j) {
+            if (order > limit) append(order, j);
+            return true;
+        });
+        __syncthreads();
+        const uint32_t t = threadIdx.x, lane = t & 63, above = shared().count, want = k - above;
+        uint32_t have = 0;
+        elements(span, s, [&](uint32_t order, uint32_t j) {
+            const bool equal = j < s.e1 && order == limit;
+            const uint64_t in_wave = __builtin_amdgcn_ballot_w64(equal);
+            __syncthreads();
+            if (lane == 0) shared().words[t >> 6] = (uint32_t)__builtin_popcountll(in_wave);
+            __syncthreads();
+            uint32_t at = have + (uint32_t)__builtin_popcountll(in_wave & ((1ull << lane) - 1));
+            for (uint32_t w = 0; w < THREADS / 64; ++w) {
+                if (w < (t >> 6)) at += shared().words[w];
+                have += shared().words[w];
+            }
+            if (equal && at < want) shared().list[above + at] = composite(order, j);
+            return have < want;
+        });
+        __syncthreads();
+        if (t == 0) shared().count = k;
+        __syncthreads();
+    }
+
+    // Keeps those of the thread's G vectors from base on that hold a logit from least (> -inf) on; hi: the largest logit.
+    // Which of their logits these are is left to sift(), where every thread looks at one.
+    template <int G> static __device__ __forceinline__ void meet(const RowSpan<T>& span, const u32x4* raw, float hi, uint32_t base, float least) {
+        if (!(hi >= least)) return;
+#pragma unroll
+        for (int u = 0; u < G; ++u) {
+            float x[N];
+            LogitVec<T>::unpack(raw[u], x);
+            if (G == 1 || largest(x) >= least) {
+                const uint32_t at = __hip_atomic_fetch_add(&shared().n_vectors, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                if (at < (uint32_t)VECTORS) {
+                    shared().vectors[at] = raw[u];
+                    shared().at[at] = span.index(base + u * THREADS + threadIdx.x);
+                }
+            }
+        }
+    }
+    static __device__ __forceinline__ void sift(float least) {
+        __syncthreads();
+        const uint32_t n = shared().n_vectors;
+        if (n <= (uint32_t)VECTORS)
+            for (uint32_t i = threadIdx.x; i < n * N; i += THREADS) {
+                const float x = LogitVec<T>::load((const T*)shared().vectors + i);
+                if (x >= least) append(order_of(x), shared().at[i / N] + i % N);
+            }
+        __syncthreads();
+    }
+    static __device__ __forceinline__ bool overflow() { return shared().n_vectors > (uint32_t)VECTORS || shared().count > (uint32_t)LIST; }
+    // A long row's k largest are collected while it is read: a threshold from the threads' first vectors holds for the
+    // whole row and lets through about as many times k logits as the row is longer than they are.
+    // The value from which logits are let through; NaN, which lets none through, where there are no k logits above -inf.
+    static __device__ __forceinline__ float early(float top, bool any, uint32_t k) {
+        bool exact;
+        const uint32_t limit = threshold(top, any, k, &exact);
+        return limit <= 0x007fffffu ? __builtin_nanf("") : logit_of(limit);
+    }
+
+    static __device__ __forceinline__ void edge(const RowSpan<T>& span, const Slice& s, float least) {
+        if (s.edge >= 0) {
+            const float x = LogitVec<T>::load(span.row + s.edge);
+            if (x >= least) append(order_of(x), (uint32_t)s.edge);
+        }
+    }
+    // Leaves at least the k largest of the slice (all of them, if it has fewer) in the list, in any order, given
+    // the threshold of the threads' largest logits.  look(least): meets the thread's vectors, every(least): the same for
+    // any least, -inf among them; top: the thread's largest logit; nan: the row holds a NaN or +inf.
+    template <typename F, typename E>
+    static __device__ __forceinline__ void select(const RowSpan<T>& span, const Slice& s, uint32_t limit, bool exact, float top, bool nan,
+                                           uint32_t k, F look, E every) {
+        if (!nan && !(exact && limit == 0x007fffffu)) {   // (-inf: a mask has left fewer than k logits)
+            const float least = limit <= 0x007fffffu ? -kInf : logit_of(limit);
+            if (limit <= 0x007fffffu) every(least);
+            else if (top >= least) look(least);
+            edge(span, s, least);
+            sift(least);
+            if (!overflow()) return;
+        }
+        select_exactly(span, s, k, limit, exact && !nan);
     }
 };
+
+// Rank of every composite of list[0 .. n); those below k go to f(rank, composite).  As many lanes as there are threads
+// for share the comparisons of one composite.
+template <int THREADS, typename F> __device__ __forceinline__ void ranked(const uint64_t* list, uint32_t n, uint32_t k, F f) {
+    uint32_t share = 1;
+    while (share < 16 && 2 * share * n <= (uint32_t)THREADS) share *= 2;
+    for (uint32_t i0 = 0; i0 < n; i0 += THREADS / share) {
+        const uint32_t i = i0 + threadIdx.x / share, part = threadIdx.x % share;
+        const uint64_t mine = i < n ? list[i] : ~0ull;
+        int rank = 0;
+        for (uint32_t j = part; j < n; j += share) rank += list[j] > mine;
+        if (share > 1) rank += __builtin_amdgcn_update_dpp(0, rank, 0xB1, 0xf, 0xf, true);
+        if (share > 2) rank += __builtin_amdgcn_update_dpp(0, rank, 0x4E, 0xf, 0xf, true);
+        if (share > 4) rank += __builtin_amdgcn_update_dpp(0, rank, 0x141, 0xf, 0xf, true);
+        if (share > 8) rank += __builtin_amdgcn_update_dpp(0, rank, 0x140, 0xf, 0xf, true);
+        if (part == 0 && i < n && (uint32_t)rank < k) f((uint32_t)rank, mine);
+    }
+}
 
 struct LogprobParams {
     const void* logits;
@@ -331,115 +695,197 @@ __device__ __forceinline__ float log_prob(float x, float m, float l, float scale
     return l == -kInf ? -kInf : (x - m) * scale - l * kLn2;
 }
 
-// Sums a row over the work-group's threads: every thread returns with m, sum, dot of the whole row (and its own top).
-template <typename T, int THREADS, bool ENTROPY>
-__device__ __forceinline__ RowSum sum_row(const RowSpan<T>& span, int32_t edge, float c, float* red) {
-    constexpr int N = LogitVec<T>::N;
-    constexpr int UNROLL = 4;
-    const uint32_t t = threadIdx.x;
-    RowSum acc;
-    acc.clear();
-    float single[1] = {-kInf};
-    if (edge >= 0) single[0] = LogitVec<T>::load(span.row + edge);
-    for (uint32_t v = t; v < span.vecs; v += THREADS * UNROLL) {
-        u32x4 raw[UNROLL];
+// The logits of a row's tokens, one per thread, fetched before the row is read: by the time its sums are known they
+// have arrived, and no thread waits for two dependent loads while the others wait for it.
+template <typename T, int THREADS> struct NamedLogits {
+    static constexpr int ROUNDS = THREADS < (int)kMaxSlots ? (int)kMaxSlots / THREADS : 1;
+    uint32_t x[ROUNDS];   // bits
+    int32_t id[ROUNDS];   // -1: none
+    // (two steps: the loads of the row go between them, so that the wait for the ids is not one for the row)
+    __device__ __forceinline__ void load_ids(const int32_t* ids, uint32_t n) {
 #pragma unroll
-        for (int u = 0; u < UNROLL; ++u)
-            if (v + u * THREADS < span.vecs) raw[u] = span.vec(v + u * THREADS);
-#pragma unroll
-        for (int u = 0; u < UNROLL; ++u)
-            if (v + u * THREADS < span.vecs) {
-                float x[N];
-                LogitVec<T>::unpack(raw[u], x);
-                acc.template add<ENTROPY>(x, c);
-            }
-    }
-    if (edge >= 0) acc.template add<ENTROPY>(single, c);
-    const float top = group_max<THREADS>(acc.top, red);
-    if (fabsf(top * c) > kWide && fabsf(top) < kInf) {
-        // logits as large as a type's lowest value (masks made of it): the largest is the reference
-        acc.sum = acc.dot = 0.f;
-        for (uint32_t v = t; v < span.vecs; v += THREADS) {
-            float x[N];
-            LogitVec<T>::unpack(span.vec(v), x);
-            acc.template add_wide<ENTROPY>(x, c, top);
+        for (int r = 0; r < ROUNDS; ++r) {
+            const uint32_t i = threadIdx.x + r * THREADS;
+            id[r] = -1;
+            if (i < n) id[r] = ids[i];
         }
-        if (edge >= 0) acc.template add_wide<ENTROPY>(single, c, top);
-        acc.ref = top;
-    } else {
-        acc.template settle<ENTROPY>(c);
-        acc.template move<ENTROPY>(group_max<THREADS>(acc.ref, red), c);
     }
-    acc.sum = group_sum<THREADS>(acc.sum, red);
-    if (ENTROPY) acc.dot = group_sum<THREADS>(acc.dot, red);
-    return acc;
+    __device__ __forceinline__ void load_logits(const RowSpan<T>& span, uint32_t vocab) {
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r) {
+            if ((uint32_t)id[r] >= vocab) id[r] = -1;
+            x[r] = 0;
+            if (id[r] >= 0) x[r] = LogitVec<T>::bits(span.row + id[r]);
+        }
+    }
+    __device__ __forceinline__ void write(float* logprob, uint32_t n, float m, float l, float scale) const {
+#pragma unroll
+        for (int r = 0; r < ROUNDS; ++r) {
+            const uint32_t i = threadIdx.x + r * THREADS;
+            if (i < n) logprob[i] = id[r] >= 0 ? log_prob(LogitVec<T>::value(x[r]), m, l, scale) : 0.f;
+        }
+    }
+};
+
+template <bool ENTROPY> __device__ __forceinline__ void write_row_sums(const LogprobParams& p, size_t row, const RowSum& r, float l) {
+    if (threadIdx.x != 0) return;
+    if (p.stats) { p.stats[2 * row] = r.m; p.stats[2 * row + 1] = l; }
+    if (ENTROPY) {
+        const float h = (l - r.dot / r.sum) * kLn2;
+        p.entropy[row] = l == -kInf || h < 0.f ? 0.f : h;   // (rounding can leave a certain row below zero)
+    }
 }
 
-// One work-group per row.
-template <typename T, int THREADS, bool ENTROPY>
-__global__ __launch_bounds__(THREADS) void token_logprobs_kernel(LogprobParams p) {
-    __shared__ float red[16];
-    __shared__ uint64_t list[512];
-    __shared__ uint32_t words[THREADS];
-    __shared__ uint32_t count;
+// One work-group per row, held in registers (NV vectors per thread) or, NV = 0, streamed.
+template <typename T, int THREADS, int NV, bool ENTROPY>
+__global__ __launch_bounds__(THREADS, NV == 0 ? 8 : 4) void token_logprobs_kernel(LogprobParams p) {
+    typedef TopSelect<T, THREADS> Top;
+    __shared__ float red[32];
+    constexpr int N = LogitVec<T>::N;
     const uint32_t t = threadIdx.x;
     const size_t row = blockIdx.x;
     const RowSpan<T> span((const T*)p.logits + row * p.stride, p.vocab);
-    const int32_t edge = span.edge(t);
-    const RowSum acc = sum_row<T, THREADS, ENTROPY>(span, edge, p.c, red);
-    const float m = acc.ref, l = log2f(acc.sum);
-    if (t == 0) {
-        if (p.stats) { p.stats[2 * row] = m; p.stats[2 * row + 1] = l; }
-        if (ENTROPY) {
-            const float h = (l - acc.dot / acc.sum) * kLn2;
-            p.entropy[row] = l == -kInf || h < 0.f ? 0.f : h;   // (rounding can leave a certain row below zero)
+    const Slice s = slice_of(span, p.vocab, 0, 1, 0, t);
+    NamedLogits<T, THREADS> named;
+    named.load_ids(p.tokens + row * p.n_tokens, p.n_tokens);
+    const uint32_t k = p.top_k;
+    typedef Held<T, THREADS, NV ? NV : 1> Registers;
+    typedef Streamed<T, THREADS> Stream;
+    Registers held;
+    RowSum r;
+    const bool any = t < s.v1 || s.edge >= 0;
+    float least = __builtin_nanf("");
+    if (NV) {
+        held.load(span, s, t);
+        named.load_logits(span, p.vocab);
+        auto publish = [&](float hi) { if (k) Top::publish(hi, any, k); };
+        auto met = [&]() { if (k) Top::find(k); };
+        r = held.template sums<ENTROPY>(s, t, p.c, red, publish, met);
+    } else {
+        named.load_logits(span, p.vocab);
+        auto early = [&](auto first) { if (k) least = Top::early(first(), any, k); };
+        auto meet = [&](auto count, const u32x4* raw, float hi, uint32_t base) {
+            Top::template meet<decltype(count)::value>(span, raw, hi, base, least);
+        };
+        r = Stream::template sums<ENTROPY>(span, s, t, p.c, red, early, meet);
+    }
+    const float l = log2f(r.sum);
+    write_row_sums<ENTROPY>(p, row, r, l);
+    named.write(p.logprob + row * p.n_tokens, p.n_tokens, r.m, l, p.scale);
+    if (k == 0) return;
+    const bool nan = r.sum != r.sum;
+    bool exact = false;
+    if (NV) {
+        if (THREADS == 64) __syncthreads();
+        const uint32_t limit = Top::found(&exact);
+        auto look = [&](float from) {
+            held.template steps<false>(s, t, [&](auto count, const u32x4* raw, uint32_t base) {
+                Top::template meet<decltype(count)::value>(span, raw, largest_of<T, decltype(count)::value>(raw), base, from);
+            });
+        };
+        auto every = [&](float from) {
+            held.each(s, t, [&](const float (&x)[N], uint32_t base) { Top::scan(x, span.index(base + t), from); });
+        };
+        Top::select(span, s, limit, exact, r.top, nan, k, look, every);
+    } else {
+        if (least == least) Top::edge(span, s, least);
+        Top::sift(least);
+        if (!(least == least) || nan || Top::overflow()) {
+            const uint32_t limit = nan ? 0u : Top::threshold(r.top, any, k, &exact);
+            auto every = [&](float from) {
+                Stream::each(span, s, t, [&](const float (&x)[N], uint32_t base) { Top::scan(x, span.index(base + t), from); });
+            };
+            Top::select(span, s, limit, exact, r.top, nan, k, every, every);
         }
     }
-    for (uint32_t i = t; i < p.n_tokens; i += THREADS) {
-        const int32_t id = p.tokens[row * p.n_tokens + i];
-        float lp = 0.f;
-        if (id >= 0 && (uint32_t)id < p.vocab) lp = log_prob(LogitVec<T>::load(span.row + id), m, l, p.scale);
-        p.logprob[row * p.n_tokens + i] = lp;
-    }
-    if (p.top_k == 0) return;
-    TopSelect<T, THREADS> top{list, words, &count};
-    top.select(span, p.vocab, edge, acc.top, t < span.vecs || edge >= 0, acc.sum != acc.sum, p.top_k);
-    const uint32_t n = count;
-    for (uint32_t i = t; i < n; i += THREADS) {
-        const uint64_t mine = list[i];
-        uint32_t rank = 0;
-        for (uint32_t j = 0; j < n; ++j) rank += list[j] > mine;
-        if (rank < p.top_k) {
-            p.top_ids[row * p.top_k + rank] = (int32_t)~(uint32_t)mine;
-            p.top_logprobs[row * p.top_k + rank] = log_prob(logit_of((uint32_t)(mine >> 32)), m, l, p.scale);
-        }
-    }
+    ranked<THREADS>(Top::shared().list, Top::shared().count, k, [&](uint32_t rank, uint64_t c) {
+        p.top_ids[row * p.top_k + rank] = (int32_t)~(uint32_t)c;
+        p.top_logprobs[row * p.top_k + rank] = log_prob(logit_of((uint32_t)(c >> 32)), r.m, l, p.scale);
+    });
 }
 
 // ---- gradients ------------------------------------------------------------------------------------------------
 // Both operators' gradients have one form.  With coefficients c_i on tokens id_i, C = sum_i c_i over the valid ones and
 // g the gradient of the entropy H:   dx_j = s ( sum_{i: id_i = j} c_i - C p_j - g p_j (ln p_j + H) ).
-struct GradParams {
-    const void* logits;
-    void* d_logits;
-    const int32_t* ids;      // [rows][n]
-    const float* stats;
-    const float *entropy, *d_entropy;   // or NULL
-    const float* d_logprob;  // coefficients [rows][n] ...
-    const void* teacher;     // ... or a teacher's logits [rows][n] and
-    const float* d_loss;     // the gradient of each row's loss
-    uint64_t stride;
-    uint32_t vocab, n, chunks, chunk_vecs;
-    int teacher_bf16;
-    float scale, c;
+struct RowGrad {
+    float m, l, c;
+    float whole;     // -s C 2^-l
+    float ent, H;    // -s g 2^-l, entropy
+    __device__ __forceinline__ void set(float m_, float l_, float c_, float minus_s_C, float minus_s_g, float H_) {
+        const float inv = exp2_fast(-l_);
+        m = m_; l = l_; c = c_; H = H_;
+        whole = minus_s_C * inv;
+        ent = minus_s_g * inv;
+    }
+    template <bool ENTROPY> __device__ __forceinline__ float at(float x) const {
+        const float t = (x - m) * c, e = exp2_fast(t);
+        float d = whole * e;
+        if (ENTROPY) d = fmaf(ent * e, fmaf(fmaxf(t, -256.f) - l, kLn2, H), d);
+        return d;
+    }
 };
 
+// Writes a slice of a row's gradient, then the entries in it that tokens name.  Equal tokens add up in slot order and the
+// first of them writes the entry.  d may be the logits themselves: the named ones are read before anything is written.
+// ids, coef: shared memory, complete.  each(f): f(x, base) for every vector of the thread.
+template <typename T, int THREADS, bool ENTROPY, typename EACH>
+__device__ __forceinline__ void write_gradient(const RowSpan<T>& span, const Slice& s, T* d, const RowGrad& g, const int32_t* ids,
+                                               const float* coef, uint32_t n, float scale, EACH each) {
+    constexpr int N = LogitVec<T>::N;
+    constexpr uint32_t ROUNDS = THREADS < (int)kMaxSlots ? kMaxSlots / THREADS : 1;
+    const uint32_t t = threadIdx.x;
+    float named[ROUNDS];
+    bool writes[ROUNDS];
+#pragma unroll
+    for (uint32_t r = 0; r < ROUNDS; ++r) {
+        const uint32_t i = t + r * THREADS;
+        writes[r] = false;
+        named[r] = 0.f;
+        if (i < n) {
+            const int32_t id = ids[i];
+            if (id >= 0 && (uint32_t)id >= s.e0 && (uint32_t)id < s.e1) {
+                const float x = LogitVec<T>::load(span.row + id);
+                float total = 0.f;
+                bool first = true;
+                for (uint32_t k = 0; k < n; ++k)
+                    if (ids[k] == id) {
+                        if (k < i) { first = false; break; }
+                        total += coef[k];
+                    }
+                writes[r] = first;
+                named[r] = fmaf(scale, total, g.template at<ENTROPY>(x));
+            }
+        }
+    }
+    __syncthreads();
+    const RowSpan<T> to = span.onto(d);
+    each([&](float (&x)[N], uint32_t base) {
+#pragma unroll
+        for (int u = 0; u < N; ++u) x[u] = g.template at<ENTROPY>(x[u]);
+        __builtin_nontemporal_store(LogitVec<T>::pack(x), (u32x4*)to.at(base, t));
+    });
+    if (s.edge >= 0) LogitVec<T>::store(d + s.edge, g.template at<ENTROPY>(LogitVec<T>::load(span.row + s.edge)));
+    __syncthreads();
+#pragma unroll
+    for (uint32_t r = 0; r < ROUNDS; ++r)
+        if (writes[r]) LogitVec<T>::store(d + ids[t + r * THREADS], named[r]);
+}
+
+// A row that nothing reaches (padding): zeros, whatever its logits hold.
+template <typename T, int THREADS> __device__ __forceinline__ void write_zeros(const RowSpan<T>& span, const Slice& s, T* d) {
+    const RowSpan<T> to = span.onto(d);
+    for (uint32_t base = s.v0; base + threadIdx.x < s.v1; base += THREADS)
+        __builtin_nontemporal_store(u32x4{0, 0, 0, 0}, (u32x4*)to.at(base, threadIdx.x));
+    if (s.edge >= 0) LogitVec<T>::store(d + s.edge, 0.f);
+}
+
+// ---- a teacher's list -----------------------------------------------------------------------------------------
 __device__ __forceinline__ float teacher_logit(const void* z, int as_bf16, size_t i) {
     return as_bf16 ? bf16_bits_to_f32(((const uint16_t*)z)[i]) : ((const float*)z)[i];
 }
 
-// Softmax of a teacher's list over its valid slots, by one wave: q[0 .. n) and returns sum q log2 q; *some: there is a
-// distribution (a valid slot above -inf).
+// Softmax of a teacher's list over its used slots, by one wave: q[0 .. n); returns sum q log2 q.  *some: there is a
+// distribution (a used slot above -inf).
 __device__ __forceinline__ float teacher_softmax(const int32_t* ids, const void* z, int as_bf16, size_t first, uint32_t n,
                                                  uint32_t vocab, float c, float* q, bool* some) {
     const uint32_t lane = threadIdx.x & 63;
@@ -449,19 +895,18 @@ __device__ __forceinline__ float teacher_softmax(const int32_t* ids, const void*
         const uint32_t i = lane + 64 * r;
         v[r] = -kInf;
         if (i < n) {
+            const float zi = teacher_logit(z, as_bf16, first + i);
             const int32_t id = ids[first + i];
-            if (id >= 0 && (uint32_t)id < vocab) v[r] = teacher_logit(z, as_bf16, first + i);
+            if (id >= 0 && (uint32_t)id < vocab) v[r] = zi;
         }
         hi = fmaxf(hi, v[r]);
     }
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) hi = fmaxf(hi, __shfl_xor(hi, d));
+    hi = wave_max(hi);
     float sum = 0.f;
 #pragma unroll
     for (uint32_t r = 0; r < kMaxSlots / 64; ++r)
-        if (lane + 64 * r < n && v[r] != -kInf) sum += exp2_fast((v[r] - hi) * c);
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d);
+        if (v[r] != -kInf) sum += exp2_fast((v[r] - hi) * c);
+    sum = wave_sum(sum);
     const float l = log2f(sum);
     float minus_entropy = 0.f;
 #pragma unroll
@@ -477,129 +922,80 @@ __device__ __forceinline__ float teacher_softmax(const int32_t* ids, const void*
             q[i] = qi;
         }
     }
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) minus_entropy += __shfl_xor(minus_entropy, d);
     *some = !(sum == 0.f);
-    return minus_entropy;
+    return wave_sum(minus_entropy);
 }
 
-struct RowGrad {
-    float m, l, c;
-    float whole;         // -s C
-    float ent, H;        // -s g, entropy
-    template <bool ENTROPY> __device__ __forceinline__ float at(float x) const {
-        const float t = (x - m) * c - l, pr = exp2_fast(t);
-        float d = whole * pr;
-        if (ENTROPY) d = fmaf(ent * pr, fmaf(fmaxf(t, -256.f), kLn2, H), d);
-        return d;
-    }
+// ---- gradients from a row's statistics ------------------------------------------------------------------------
+struct GradParams {
+    const void* logits;
+    void* d_logits;
+    const int32_t* ids;      // [rows][n]
+    const float* stats;
+    const float *entropy, *d_entropy;   // or NULL
+    const float* d_logprob;  // coefficients [rows][n] ...
+    const void* teacher;     // ... or a teacher's logits [rows][n] and
+    const float* d_loss;     // the gradient of each row's loss
+    uint64_t stride;
+    uint32_t vocab, n, parts, each;
+    int teacher_bf16;
+    float scale, c;
 };
 
-// Writes vectors [v0, v1) (and the edge elements if `edges`) of a row's gradient, then the entries that tokens name.
-// Same tokens add up in slot order, and the first of them writes the entry.  d may be x itself: the named logits are
-// read before anything is written.
-template <typename T, int THREADS, bool ENTROPY>
-__device__ __forceinline__ void write_gradient(const RowSpan<T>& span, T* d, uint32_t v0, uint32_t v1, bool edges, bool zero,
-                                               const RowGrad& g, const int32_t* ids, const float* coef, uint32_t n,
-                                               uint32_t vocab, float s) {
-    constexpr int N = LogitVec<T>::N;
-    const uint32_t t = threadIdx.x;
-    const int32_t edge = edges ? span.edge(t) : -1;
-    if (zero) {   // nothing reaches this row (padding): its logits, whatever they hold, are not read
-        for (uint32_t v = v0 + t; v < v1; v += THREADS) *(u32x4*)(d + span.index(v)) = u32x4{0, 0, 0, 0};
-        if (edge >= 0) LogitVec<T>::store(d + edge, 0.f);
-        return;
-    }
-    constexpr uint32_t ROUNDS = kMaxSlots / THREADS > 0 ? kMaxSlots / THREADS : 1;
-    float named[ROUNDS];
-    bool writes[ROUNDS];
-    const uint32_t first = span.index(v0), last = span.index(v1);
-#pragma unroll
-    for (uint32_t r = 0; r < ROUNDS; ++r) {
-        const uint32_t i = t + r * THREADS;
-        writes[r] = false;
-        if (i < n) {
-            const int32_t id = ids[i];
-            writes[r] = id >= 0 && (uint32_t)id < vocab &&
-                        (((uint32_t)id >= first && (uint32_t)id < last) ||
-                         (edges && ((uint32_t)id < span.head || (uint32_t)id >= span.index(span.vecs))));
-            if (writes[r]) {
-                float total = 0.f;
-                for (uint32_t k = 0; k < n; ++k)
-                    if (ids[k] == id) {
-                        if (k < i) { writes[r] = false; break; }
-                        total += coef[k];
-                    }
-                if (writes[r]) named[r] = fmaf(s, total, g.template at<ENTROPY>(LogitVec<T>::load(span.row + id)));
-            }
-        }
-    }
-    __syncthreads();
-    for (uint32_t v = v0 + t; v < v1; v += THREADS) {
-        float x[N];
-        LogitVec<T>::unpack(span.vec(v), x);
-#pragma unroll
-        for (int u = 0; u < N; ++u) x[u] = g.template at<ENTROPY>(x[u]);
-        *(u32x4*)(d + span.index(v)) = LogitVec<T>::pack(x);
-    }
-    if (edge >= 0) LogitVec<T>::store(d + edge, g.template at<ENTROPY>(LogitVec<T>::load(span.row + edge)));
-    __syncthreads();
-#pragma unroll
-    for (uint32_t r = 0; r < ROUNDS; ++r)
-        if (writes[r]) LogitVec<T>::store(d + ids[t + r * THREADS], named[r]);
-}
+constexpr int kGradThreads = 256, kGradVecs = 4;
 
-template <typename T, int THREADS, bool ENTROPY, bool TEACHER>
-__global__ __launch_bounds__(THREADS) void logit_gradient_kernel(GradParams p) {
-    __shared__ float red[16];
+// One work-group per kGradThreads * kGradVecs vectors of a row.
+template <typename T, bool ENTROPY, bool TEACHER>
+__global__ __launch_bounds__(kGradThreads) void logit_gradient_kernel(GradParams p) {
+    constexpr int THREADS = kGradThreads;
+    __shared__ float red[2 * THREADS / 64];
     __shared__ float coef[kMaxSlots];
     __shared__ int32_t ids[kMaxSlots];
+    __shared__ uint32_t some_teacher;
     const uint32_t t = threadIdx.x;
-    const size_t row = blockIdx.x / p.chunks;
-    const uint32_t chunk = blockIdx.x % p.chunks;
+    const size_t row = blockIdx.x / p.parts;
     const RowSpan<T> span((const T*)p.logits + row * p.stride, p.vocab);
-    const uint32_t v0 = chunk * p.chunk_vecs < span.vecs ? chunk * p.chunk_vecs : span.vecs;
-    const uint32_t v1 = v0 + p.chunk_vecs < span.vecs ? v0 + p.chunk_vecs : span.vecs;
-    const float l = p.stats[2 * row + 1];
-    RowGrad g;
-    g.m = p.stats[2 * row];
-    g.l = l;
-    g.c = p.c;
-    g.ent = ENTROPY ? -p.scale * p.d_entropy[row] : 0.f;
-    g.H = ENTROPY ? p.entropy[row] : 0.f;
+    const Slice s = slice_of(span, p.vocab, blockIdx.x % p.parts, p.parts, p.each, t);
+    T* const d = (T*)p.d_logits + row * p.stride;
+    const float m = p.stats[2 * row], l = p.stats[2 * row + 1];
+    const float ent = ENTROPY ? -p.scale * p.d_entropy[row] : 0.f, H = ENTROPY ? p.entropy[row] : 0.f;
     float C = 0.f, any = 0.f;
-    const float w = TEACHER ? p.d_loss[row] / (p.scale * p.scale) : 0.f;
     if (TEACHER) {
+        const float w = p.d_loss[row] / (p.scale * p.scale);
         if (t < 64) {
             bool some;
             teacher_softmax(p.ids, p.teacher, p.teacher_bf16, row * p.n, p.n, p.vocab, p.c, coef, &some);
-            if (t == 0) red[0] = some ? 1.f : 0.f;
+            if (t == 0) some_teacher = some ? 1u : 0u;
         }
         __syncthreads();
-        if (red[0] != 0.f && w != 0.f) { C = -w; any = 1.f; }
-        __syncthreads();
-    }
-    for (uint32_t i = t; i < p.n; i += THREADS) {
-        const int32_t id = p.ids[row * p.n + i];
-        ids[i] = id;
-        if (TEACHER) {
+        for (uint32_t i = t; i < p.n; i += THREADS) {
+            ids[i] = p.ids[row * p.n + i];
             coef[i] *= -w;
-        } else {
-            const float v = id >= 0 && (uint32_t)id < p.vocab ? p.d_logprob[row * p.n + i] : 0.f;
-            coef[i] = v;
-            C += v;
-            if (v != 0.f) any = 1.f;
         }
+        C = -w;
+        any = some_teacher ? w : 0.f;
+    } else {
+        for (uint32_t i = t; i < p.n; i += THREADS) {
+            const int32_t id = p.ids[row * p.n + i];
+            const float v = p.d_logprob[row * p.n + i];
+            const bool inside = id >= 0 && (uint32_t)id < p.vocab;
+            ids[i] = id;
+            coef[i] = inside ? v : 0.f;
+            if (inside) { C += v; any += v != 0.f ? 1.f : 0.f; }
+        }
+        group_sum<THREADS, true>(C, any, red);
+        if (ent != 0.f) any = 1.f;
     }
-    if (!TEACHER) {
-        C = group_sum<THREADS>(C, red);
-        any = group_max<THREADS>(any, red);
-        if (g.ent != 0.f) any = 1.f;
+    if (any == 0.f || l == -kInf) {
+        write_zeros<T, THREADS>(span, s, d);
+        return;
     }
-    __syncthreads();
-    g.whole = -p.scale * C;
-    write_gradient<T, THREADS, ENTROPY>(span, (T*)p.d_logits + row * p.stride, v0, v1, chunk == 0,
-                                        any == 0.f || l == -kInf, g, ids, coef, p.n, p.vocab, p.scale);
+    Held<T, THREADS, kGradVecs> held;
+    held.load(span, s, t);
+    RowGrad g;
+    g.set(m, l, p.c, -p.scale * C, ent, H);
+    __syncthreads();   // ids and coef are complete
+    write_gradient<T, THREADS, ENTROPY>(span, s, d, g, ids, coef, p.n, p.scale, [&](auto f) { held.each(s, t, f); });
 }
 
 // ---- distillation ---------------------------------------------------------------------------------------------
@@ -616,67 +1012,101 @@ struct DistillParams {
     float scale, c;
 };
 
-// One work-group per row: the student's softmax sum, the loss over the teacher's slots, and (GRAD) the gradient in a
-// second sweep over the row.
-template <typename T, int THREADS, bool GRAD>
-__global__ __launch_bounds__(THREADS) void distill_kernel(DistillParams p) {
-    __shared__ float red[16];
+// Loss over a teacher's slots from the student's statistics, by one wave: q [n] in shared memory, *some as above.
+template <typename T>
+__device__ __forceinline__ float teacher_loss(const DistillParams& p, size_t row, const RowSpan<T>& span, float m, float l, float* q,
+                                              bool* some) {
+    const float minus_entropy = teacher_softmax(p.ids, p.teacher, p.teacher_bf16, row * p.n, p.n, p.vocab, p.c, q, some);
+    float cross = 0.f;
+    for (uint32_t i = threadIdx.x & 63; i < p.n; i += 64)
+        if (!(q[i] <= 0.f)) cross += q[i] * log_prob(LogitVec<T>::load(span.row + p.ids[row * p.n + i]), m, l, p.scale);
+    cross = wave_sum(cross);
+    return *some ? (minus_entropy * kLn2 - cross) / (p.scale * p.scale) : 0.f;
+}
+
+// One work-group per row, held in registers (NV vectors per thread) or, NV = 0, streamed: the student's sums, the loss,
+// and (GRAD) the gradient, for which a held row is not read again.
+template <typename T, int THREADS, int NV, bool GRAD>
+__global__ __launch_bounds__(THREADS, THREADS == 1024 && NV == 8 ? 8 : 4) void distill_kernel(DistillParams p) {
+    __shared__ float red[32];
     __shared__ float q[kMaxSlots];
     __shared__ int32_t ids[kMaxSlots];
-    __shared__ uint32_t has_teacher;
+    __shared__ uint32_t some_teacher;
     const uint32_t t = threadIdx.x;
     const size_t row = blockIdx.x;
     const RowSpan<T> span((const T*)p.logits + row * p.stride, p.vocab);
-    float valid = 0.f;
+    const Slice s = slice_of(span, p.vocab, 0, 1, 0, t);
+    T* const d = GRAD ? (T*)p.d_logits + row * p.stride : nullptr;
+    float used = 0.f;
     for (uint32_t i = t; i < p.n; i += THREADS) {
         const int32_t id = p.ids[row * p.n + i];
         ids[i] = id;
-        if (id >= 0 && (uint32_t)id < p.vocab) valid = 1.f;
+        if (id >= 0 && (uint32_t)id < p.vocab) used = 1.f;
     }
-    valid = group_max<THREADS>(valid, red);
-    RowGrad g;
-    g.m = g.l = -kInf;
-    g.c = p.c;
-    g.ent = g.H = 0.f;
-    bool some = false;
-    if (valid != 0.f) {   // (a row without a slot is padding: its logits are not read)
-        const RowSum acc = sum_row<T, THREADS, false>(span, span.edge(t), p.c, red);
-        g.m = acc.ref;
-        g.l = log2f(acc.sum);
-        float loss = 0.f;
-        if (t < 64) {
-            loss = teacher_softmax(p.ids, p.teacher, p.teacher_bf16, row * p.n, p.n, p.vocab, p.c, q, &some);
-            float cross = 0.f;
-            for (uint32_t i = t; i < p.n; i += 64)
-                if (q[i] > 0.f || q[i] != q[i]) cross += q[i] * log_prob(LogitVec<T>::load(span.row + ids[i]), g.m, g.l, p.scale);
-#pragma unroll
-            for (int d = 32; d >= 1; d >>= 1) cross += __shfl_xor(cross, d);
-            loss = some ? (loss * kLn2 - cross) / (p.scale * p.scale) : 0.f;
-            if (t == 0) {
-                p.row_loss[row] = loss;
-                has_teacher = some ? 1u : 0u;
-            }
+    used = group_max<THREADS>(used, red, []() {});
+    if (used == 0.f) {   // no slot (padding): the logits are not read
+        if (t == 0) {
+            p.row_loss[row] = 0.f;
+            if (p.stats) { p.stats[2 * row] = -kInf; p.stats[2 * row + 1] = -kInf; }
         }
-        __syncthreads();
-        some = has_teacher != 0u;
-    } else if (t == 0) {
-        p.row_loss[row] = 0.f;
+        if (GRAD) write_zeros<T, THREADS>(span, s, d);
+        return;
     }
-    if (t == 0 && p.stats) { p.stats[2 * row] = g.m; p.stats[2 * row + 1] = g.l; }
+    Held<T, THREADS, NV ? NV : 1> held;
+    RowSum r;
+    if (NV) {
+        held.load(span, s, t);
+        r = held.template sums<false>(s, t, p.c, red, [](float) {}, []() {});
+    } else {
+        r = Streamed<T, THREADS>::template sums<false>(span, s, t, p.c, red, [](auto) {}, [](auto, const u32x4*, float, uint32_t) {});
+    }
+    const float l = log2f(r.sum);
+    if (t < 64) {
+        bool some;
+        const float loss = teacher_loss<T>(p, row, span, r.m, l, q, &some);
+        if (t == 0) {
+            p.row_loss[row] = loss;
+            if (p.stats) { p.stats[2 * row] = r.m; p.stats[2 * row + 1] = l; }
+            some_teacher = some ? 1u : 0u;
+        }
+    }
     if (GRAD) {
         const float w = p.d_loss[row] / (p.scale * p.scale);
+        __syncthreads();
+        if (!some_teacher || w == 0.f || l == -kInf) {
+            write_zeros<T, THREADS>(span, s, d);
+            return;
+        }
         for (uint32_t i = t; i < p.n; i += THREADS) q[i] *= -w;
         __syncthreads();
-        g.whole = p.scale * w;
-        write_gradient<T, THREADS, false>(span, (T*)p.d_logits + row * p.stride, 0, span.vecs, true,
-                                          !some || w == 0.f || g.l == -kInf, g, ids, q, p.n, p.vocab, p.scale);
+        RowGrad g;
+        g.set(r.m, l, p.c, p.scale * w, 0.f, 0.f);
+        write_gradient<T, THREADS, false>(span, s, d, g, ids, q, p.n, p.scale, [&](auto f) {
+            if (NV) held.each(s, t, f);
+            else Streamed<T, THREADS>::each(span, s, t, f);
+        });
     }
 }
 
-// Threads of a row's work-group: a wave where a row is a few vectors per lane, more waves the longer it is.
-static inline int row_threads(uint32_t vocab, int dtype) {
+// How a row is spread over a work-group: threads, and vectors per thread held in registers (0: streamed).
+struct RowShape { int threads, vecs; };
+static inline RowShape logprobs_shape(uint32_t vocab, int dtype) {
     const uint32_t vecs = vocab / (dtype == SFB_BF16 ? 8u : 4u);
-    return vecs <= 512 ? 64 : vecs <= 16384 ? 256 : 1024;
+    if (vecs <= 64) return {64, 1};
+    if (vecs <= 256) return {64, 4};
+    if (vecs <= 1024) return {256, 4};
+    return {512, 0};
+}
+static inline RowShape distill_shape(uint32_t vocab, int dtype) {
+    const uint32_t vecs = vocab / (dtype == SFB_BF16 ? 8u : 4u);
+    if (vecs <= 64) return {64, 1};
+    if (vecs <= 256) return {64, 4};
+    if (vecs <= 1024) return {256, 4};
+    if (vecs <= 2048) return {256, 8};
+    if (vecs <= 4096) return {512, 8};
+    if (vecs <= 8192) return {1024, 8};
+    if (vecs <= 16384) return {1024, 16};
+    return {1024, 0};
 }
 
 static inline int check_logits(const void* logits, int dtype, uint64_t rows, uint32_t vocab, uint64_t stride, float scale,
@@ -698,13 +1128,6 @@ static inline bool misaligned4(const void* a, const void* b = nullptr, const voi
 
 using namespace sfb;
 
-#define SFB_ROW_THREADS(CALL)                                          \
-    switch (row_threads(vocab, dtype)) {                               \
-    case 64: CALL(64); break;                                          \
-    case 256: CALL(256); break;                                        \
-    default: CALL(1024); break;                                        \
-    }
-
 extern "C" int sfb_token_logprobs(sfb_stream_t stream, float* logprob, float* entropy, float* stats, int32_t* top_ids,
                                   float* top_logprobs, const void* logits, int dtype, const int32_t* tokens, uint64_t rows,
                                   uint32_t vocab, uint64_t row_stride, uint32_t n_tokens, uint32_t top_k, float scale,
@@ -720,40 +1143,42 @@ extern "C" int sfb_token_logprobs(sfb_stream_t stream, float* logprob, float* en
                     scale * kLog2e};
     hipStream_t s = (hipStream_t)stream;
     clear_stale_error();
-#define SFB_LP(TH)                                                                                          \
-    do {                                                                                                    \
-        if (dtype == SFB_F32) {                                                                             \
-            if (entropy) token_logprobs_kernel<float, TH, true><<<dim3((uint32_t)rows), TH, 0, s>>>(p);     \
-            else token_logprobs_kernel<float, TH, false><<<dim3((uint32_t)rows), TH, 0, s>>>(p);            \
-        } else {                                                                                            \
-            if (entropy) token_logprobs_kernel<__bf16, TH, true><<<dim3((uint32_t)rows), TH, 0, s>>>(p);    \
-            else token_logprobs_kernel<__bf16, TH, false><<<dim3((uint32_t)rows), TH, 0, s>>>(p);           \
-        }                                                                                                   \
+    const RowShape shape = logprobs_shape(vocab, dtype);
+    const dim3 grid((uint32_t)rows);
+#define SFB_LP_AS(T, ENT)                                                                                        \
+    do {                                                                                                         \
+        if (shape.threads == 64 && shape.vecs == 1) token_logprobs_kernel<T, 64, 1, ENT><<<grid, 64, 0, s>>>(p); \
+        else if (shape.threads == 64) token_logprobs_kernel<T, 64, 4, ENT><<<grid, 64, 0, s>>>(p);               \
+        else if (shape.threads == 256) token_logprobs_kernel<T, 256, 4, ENT><<<grid, 256, 0, s>>>(p);            \
+        else token_logprobs_kernel<T, 512, 0, ENT><<<grid, 512, 0, s>>>(p);                                      \
     } while (0)
-    SFB_ROW_THREADS(SFB_LP)
+#define SFB_LP(T)                        \
+    do {                                 \
+        if (entropy) SFB_LP_AS(T, true); \
+        else SFB_LP_AS(T, false);        \
+    } while (0)
+    if (dtype == SFB_F32) SFB_LP(float);
+    else SFB_LP(__bf16);
+#undef SFB_LP_AS
 #undef SFB_LP
     return launch_status();
 }
 
-// Vectors of a row that one work-group of the backward pass writes.
-static inline uint32_t grad_chunk_vecs(uint32_t) { return 1024; }
-
 static int launch_gradient(hipStream_t s, GradParams& p, int dtype, uint64_t rows, bool entropy, bool teacher) {
-    const uint32_t per = dtype == SFB_BF16 ? 8 : 4;
-    p.chunk_vecs = grad_chunk_vecs(p.vocab);
-    p.chunks = (p.vocab / per + p.chunk_vecs - 1) / p.chunk_vecs;
-    if (p.chunks == 0) p.chunks = 1;
-    if (rows * p.chunks > 0x7fffffffull) return SFB_ERR_SHAPE;
-    const dim3 grid((uint32_t)(rows * p.chunks));
+    const uint32_t vecs = p.vocab / (dtype == SFB_BF16 ? 8u : 4u);
+    p.each = kGradThreads * kGradVecs;
+    p.parts = vecs == 0 ? 1 : (vecs + p.each - 1) / p.each;
+    if (rows * p.parts > 0x7fffffffull) return SFB_ERR_SHAPE;
+    const dim3 grid((uint32_t)(rows * p.parts));
     clear_stale_error();
     if (dtype == SFB_F32) {
-        if (teacher) logit_gradient_kernel<float, 256, false, true><<<grid, 256, 0, s>>>(p);
-        else if (entropy) logit_gradient_kernel<float, 256, true, false><<<grid, 256, 0, s>>>(p);
-        else logit_gradient_kernel<float, 256, false, false><<<grid, 256, 0, s>>>(p);
+        if (teacher) logit_gradient_kernel<float, false, true><<<grid, kGradThreads, 0, s>>>(p);
+        else if (entropy) logit_gradient_kernel<float, true, false><<<grid, kGradThreads, 0, s>>>(p);
+        else logit_gradient_kernel<float, false, false><<<grid, kGradThreads, 0, s>>>(p);
     } else {
-        if (teacher) logit_gradient_kernel<__bf16, 256, false, true><<<grid, 256, 0, s>>>(p);
-        else if (entropy) logit_gradient_kernel<__bf16, 256, true, false><<<grid, 256, 0, s>>>(p);
-        else logit_gradient_kernel<__bf16, 256, false, false><<<grid, 256, 0, s>>>(p);
+        if (teacher) logit_gradient_kernel<__bf16, false, true><<<grid, kGradThreads, 0, s>>>(p);
+        else if (entropy) logit_gradient_kernel<__bf16, true, false><<<grid, kGradThreads, 0, s>>>(p);
+        else logit_gradient_kernel<__bf16, false, false><<<grid, kGradThreads, 0, s>>>(p);
     }
     return launch_status();
 }
@@ -792,17 +1217,27 @@ extern "C" int sfb_distillation_loss(sfb_stream_t stream, float* row_loss, float
                     teacher_dtype == SFB_BF16 ? 1 : 0, scale, scale * kLog2e};
     hipStream_t s = (hipStream_t)stream;
     clear_stale_error();
-#define SFB_DL(TH)                                                                                     \
-    do {                                                                                               \
-        if (dtype == SFB_F32) {                                                                        \
-            if (d_logits) distill_kernel<float, TH, true><<<dim3((uint32_t)rows), TH, 0, s>>>(p);      \
-            else distill_kernel<float, TH, false><<<dim3((uint32_t)rows), TH, 0, s>>>(p);              \
-        } else {                                                                                       \
-            if (d_logits) distill_kernel<__bf16, TH, true><<<dim3((uint32_t)rows), TH, 0, s>>>(p);     \
-            else distill_kernel<__bf16, TH, false><<<dim3((uint32_t)rows), TH, 0, s>>>(p);             \
-        }                                                                                              \
+    const RowShape shape = distill_shape(vocab, dtype);
+    const dim3 grid((uint32_t)rows);
+#define SFB_DL_AS(T, GRAD)                                                                                         \
+    do {                                                                                                           \
+        if (shape.threads == 64 && shape.vecs == 1) distill_kernel<T, 64, 1, GRAD><<<grid, 64, 0, s>>>(p);         \
+        else if (shape.threads == 64) distill_kernel<T, 64, 4, GRAD><<<grid, 64, 0, s>>>(p);                       \
+        else if (shape.threads == 256 && shape.vecs == 4) distill_kernel<T, 256, 4, GRAD><<<grid, 256, 0, s>>>(p); \
+        else if (shape.threads == 256) distill_kernel<T, 256, 8, GRAD><<<grid, 256, 0, s>>>(p);                    \
+        else if (shape.threads == 512) distill_kernel<T, 512, 8, GRAD><<<grid, 512, 0, s>>>(p);                    \
+        else if (shape.vecs == 8) distill_kernel<T, 1024, 8, GRAD><<<grid, 1024, 0, s>>>(p);                       \
+        else if (shape.vecs == 16) distill_kernel<T, 1024, 16, GRAD><<<grid, 1024, 0, s>>>(p);                     \
+        else distill_kernel<T, 1024, 0, GRAD><<<grid, 1024, 0, s>>>(p);                                            \
     } while (0)
-    SFB_ROW_THREADS(SFB_DL)
+#define SFB_DL(T)                         \
+    do {                                  \
+        if (d_logits) SFB_DL_AS(T, true); \
+        else SFB_DL_AS(T, false);         \
+    } while (0)
+    if (dtype == SFB_F32) SFB_DL(float);
+    else SFB_DL(__bf16);
+#undef SFB_DL_AS
 #undef SFB_DL
     return launch_status();
 }
