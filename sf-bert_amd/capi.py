@@ -902,22 +902,27 @@ _LOGIT_ARGS = {
 _logit_entries = {}
 
 
-def _logit_call(name, *args):
+def _logit_call(name, stream, *args):
     fn = _logit_entries.get(name)
     if fn is None:   # with argument types plain numbers are converted without a ctypes object for each
         fn = getattr(lib, name)
         fn.argtypes = _LOGIT_ARGS[name]
         _logit_entries[name] = fn
-    _check(fn(_stream(), *args), name)
+    status = fn(stream, *args)
+    if status:
+        raise SfbError(status, name)
 
 
-def _require_device(*tensors):
-    """Launches go to the current device: tensors of another one (or of the host) are refused."""
+def _stream_for(*tensors):
+    """The current stream of the current device, to which launches go; tensors of another device (or of the host) are
+    refused."""
     import torch
     here = torch.cuda.current_device()
     for t in tensors:
-        if t is not None and (not t.is_cuda or t.device.index != here):
+        if t is not None and t.get_device() != here:
             raise SfbError(8, "tensor on %s, current device cuda:%d" % (t.device, here))
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)   # (the handle without a Stream object around it)
+    return raw(here) if raw is not None else torch.cuda.current_stream().cuda_stream
 
 
 def _logit_rows(logits):
@@ -925,13 +930,11 @@ def _logit_rows(logits):
     if logits.dim() != 2:
         raise SfbError(4, "logits of %d dimensions" % logits.dim())
     rows, vocab = logits.shape
-    if rows == 0 or vocab == 0:
-        raise SfbError(4, "logits of shape %s" % (tuple(logits.shape),))
     stride, step = logits.stride()
-    if rows == 1:
-        stride = max(stride, vocab)
-    if (step != 1 and vocab > 1) or stride < vocab:
-        raise SfbError(4, "logits with strides %s" % (logits.stride(),))
+    if rows == 1 and stride < vocab:
+        stride = vocab
+    if rows == 0 or vocab == 0 or stride < vocab or (step != 1 and vocab > 1):
+        raise SfbError(4, "logits of shape %s with strides %s" % (tuple(logits.shape), logits.stride()))
     return _dtype_code(logits), rows, vocab, stride
 
 
@@ -939,7 +942,7 @@ def _small(t, shape, dtype, what):
     """Pointer of a contiguous tensor of the given shape and type (None: NULL)."""
     if t is None:
         return None
-    if tuple(t.shape) != tuple(shape) or not t.is_contiguous():
+    if t.shape != shape or not t.is_contiguous():
         raise SfbError(4, "%s of shape %s, strides %s (expected %s)" % (what, tuple(t.shape), t.stride(), tuple(shape)))
     if t.dtype != dtype:
         raise SfbError(5, "%s of %s" % (what, t.dtype))
@@ -961,7 +964,16 @@ def _like_logits(logits, stride, out):
 def _logit_workspace(workspace):
     if workspace is None:
         return None, 0
+    if not workspace.is_contiguous():
+        raise SfbError(4, "non-contiguous workspace")
     return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+def _tokens(tokens, rows):
+    """(pointer, tokens per row) of int32 [rows] or [rows, n]"""
+    import torch
+    n = 1 if tokens.dim() == 1 else tokens.shape[-1]
+    return _small(tokens, (rows,) if tokens.dim() == 1 else (rows, n), torch.int32, "tokens"), n
 
 
 def token_logprobs(logits, tokens=None, top_k=0, scale=1.0, entropy=False, workspace=None):
@@ -969,28 +981,34 @@ def token_logprobs(logits, tokens=None, top_k=0, scale=1.0, entropy=False, works
     (sfb_token_logprobs).  logits [rows, vocab] fp32 or bf16 (rows may be further apart); tokens int32 [rows] or
     [rows, n], None for none; workspace: zero-filled uint8 tensor of LOGIT_WORKSPACE_BYTES that the caller keeps, lets
     few long rows be cut over the device.  Returns a dict: stats [rows, 2] (for the backward pass); logprob in
-    tokens' shape; entropy [rows]; top_ids int32 and top_logprobs [rows, top_k]; those not asked for are left out."""
+    tokens' shape; entropy [rows]; top_ids int32 and top_logprobs [rows, top_k]; those not asked for are left out.
+    The results are parts of one allocation."""
     import torch
     code, rows, vocab, stride = _logit_rows(logits)
-    _require_device(logits, tokens, workspace)
-    dev, f32 = logits.device, torch.float32
-    out = Luts(stats=torch.empty((rows, 2), dtype=f32, device=dev))
+    stream = _stream_for(logits, tokens, workspace)
     n, tok, lp, ent, ids, top = 0, None, None, None, None, None
     if tokens is not None:
-        n = 1 if tokens.dim() == 1 else tokens.shape[-1]
-        tok = _small(tokens, (rows,) if tokens.dim() == 1 else (rows, n), torch.int32, "tokens")
-        out["logprob"] = torch.empty(tokens.shape, dtype=f32, device=dev)
-        lp = out["logprob"].data_ptr()
-    if entropy:
-        out["entropy"] = torch.empty(rows, dtype=f32, device=dev)
-        ent = out["entropy"].data_ptr()
+        tok, n = _tokens(tokens, rows)
+    if top_k < 0:
+        raise SfbError(4, "top_k of %d" % top_k)
+    # one buffer: stats, top_logprobs, top_ids, logprob, entropy (each a whole number of floats per row)
+    buffer = torch.empty(rows * (2 + 2 * top_k + n + (1 if entropy else 0)), dtype=torch.float32, device=logits.device)
+    base, at = buffer.data_ptr(), 2 * rows
+    out = Luts(stats=buffer.as_strided((rows, 2), (2, 1), 0))
     if top_k:
-        out["top_ids"] = torch.empty((rows, top_k), dtype=torch.int32, device=dev)
-        out["top_logprobs"] = torch.empty((rows, top_k), dtype=f32, device=dev)
-        ids, top = out["top_ids"].data_ptr(), out["top_logprobs"].data_ptr()
+        out["top_logprobs"] = buffer.as_strided((rows, top_k), (top_k, 1), at)
+        top, at = base + 4 * at, at + rows * top_k
+        out["top_ids"] = buffer.as_strided((rows, top_k), (top_k, 1), at).view(torch.int32)
+        ids, at = base + 4 * at, at + rows * top_k
+    if tokens is not None:
+        out["logprob"] = buffer.as_strided(tokens.shape, tokens.stride(), at)
+        lp, at = base + 4 * at, at + rows * n
+    if entropy:
+        out["entropy"] = buffer.as_strided((rows,), (1,), at)
+        ent = base + 4 * at
     ws, ws_bytes = _logit_workspace(workspace)
-    _logit_call("sfb_token_logprobs", lp, ent, out["stats"].data_ptr(), ids, top, logits.data_ptr(), code, tok, rows, vocab,
-                stride, n, top_k, scale, ws, ws_bytes)
+    _logit_call("sfb_token_logprobs", stream, lp, ent, base, ids, top, logits.data_ptr(), code, tok, rows, vocab, stride, n,
+                top_k, scale, ws, ws_bytes)
     return out
 
 
@@ -999,19 +1017,16 @@ def token_logprobs_backward(logits, tokens, stats, d_logprob=None, entropy=None,
     stats (and entropy, where d_entropy is given); out may be the logits themselves."""
     import torch
     code, rows, vocab, stride = _logit_rows(logits)
-    _require_device(logits, tokens, stats, d_logprob, entropy, d_entropy, out)
+    stream = _stream_for(logits, tokens, stats, d_logprob, entropy, d_entropy, out)
     n, f32 = 0, torch.float32
     tok = grad = None
     if d_logprob is not None:
         if tokens is None:
             raise SfbError(1, "tokens")
-        shape = tuple(tokens.shape) if tokens.dim() != 1 else (rows,)
-        n = 1 if tokens.dim() == 1 else tokens.shape[-1]
-        if tokens.dim() > 2 or shape[0] != rows:
-            raise SfbError(4, "tokens of shape %s" % (tuple(tokens.shape),))
-        tok, grad = _small(tokens, shape, torch.int32, "tokens"), _small(d_logprob, shape, f32, "d_logprob")
+        tok, n = _tokens(tokens, rows)
+        grad = _small(d_logprob, tokens.shape, f32, "d_logprob")
     out = _like_logits(logits, stride, out)
-    _logit_call("sfb_token_logprobs_backward", out.data_ptr(), logits.data_ptr(), code, tok,
+    _logit_call("sfb_token_logprobs_backward", stream, out.data_ptr(), logits.data_ptr(), code, tok,
                 _small(stats, (rows, 2), f32, "stats"), _small(entropy, (rows,), f32, "entropy"), grad,
                 _small(d_entropy, (rows,), f32, "d_entropy"), rows, vocab, stride, n, scale)
     return out
@@ -1027,22 +1042,23 @@ def _teacher(teacher_ids, teacher_logits, rows):
 def distillation_loss(logits, teacher_ids, teacher_logits, scale=1.0, d_loss=None, out=None, workspace=None):
     """Divergence of softmax(scale * logits) from a teacher's top logits, per row (sfb_distillation_loss).  teacher_ids
     int32 and teacher_logits fp32 or bf16 [rows, slots]; ids outside the vocabulary are unused slots.  Returns a dict:
-    row_loss [rows], stats [rows, 2], and with d_loss [rows] (the gradient of each row's loss) also d_logits, written
+    row_loss [rows], stats [rows, 2] (parts of one allocation), and with d_loss [rows] (the gradient of each row's loss) also d_logits, written
     to out (which may be the logits themselves) if given.  workspace as for token_logprobs."""
     import torch
     code, rows, vocab, stride = _logit_rows(logits)
-    _require_device(logits, teacher_ids, teacher_logits, d_loss, out, workspace)
+    stream = _stream_for(logits, teacher_ids, teacher_logits, d_loss, out, workspace)
     if out is not None and d_loss is None:
         raise SfbError(1, "d_loss")
     ids, z, z_code, slots = _teacher(teacher_ids, teacher_logits, rows)
-    got = Luts(row_loss=torch.empty(rows, dtype=torch.float32, device=logits.device),
-               stats=torch.empty((rows, 2), dtype=torch.float32, device=logits.device))
+    buffer = torch.empty(3 * rows, dtype=torch.float32, device=logits.device)
+    base = buffer.data_ptr()
+    got = Luts(row_loss=buffer.as_strided((rows,), (1,), 2 * rows), stats=buffer.as_strided((rows, 2), (2, 1), 0))
     grad = None
     if d_loss is not None:
         got["d_logits"] = _like_logits(logits, stride, out)
         grad = got["d_logits"].data_ptr()
     ws, ws_bytes = _logit_workspace(workspace)
-    _logit_call("sfb_distillation_loss", got["row_loss"].data_ptr(), got["stats"].data_ptr(), grad, logits.data_ptr(), code,
+    _logit_call("sfb_distillation_loss", stream, base + 8 * rows, base, grad, logits.data_ptr(), code,
                 ids, z, z_code, _small(d_loss, (rows,), torch.float32, "d_loss"), rows, vocab, stride, slots, scale, ws,
                 ws_bytes)
     return got
@@ -1052,10 +1068,10 @@ def distillation_loss_backward(logits, teacher_ids, teacher_logits, stats, d_los
     """d_logits of sum d_loss * row_loss from distillation_loss's stats (sfb_distillation_loss_backward)."""
     import torch
     code, rows, vocab, stride = _logit_rows(logits)
-    _require_device(logits, teacher_ids, teacher_logits, stats, d_loss, out)
+    stream = _stream_for(logits, teacher_ids, teacher_logits, stats, d_loss, out)
     ids, z, z_code, slots = _teacher(teacher_ids, teacher_logits, rows)
     out = _like_logits(logits, stride, out)
-    _logit_call("sfb_distillation_loss_backward", out.data_ptr(), logits.data_ptr(), code, ids, z, z_code,
+    _logit_call("sfb_distillation_loss_backward", stream, out.data_ptr(), logits.data_ptr(), code, ids, z, z_code,
                 _small(stats, (rows, 2), torch.float32, "stats"), _small(d_loss, (rows,), torch.float32, "d_loss"), rows,
                 vocab, stride, slots, scale)
     return out

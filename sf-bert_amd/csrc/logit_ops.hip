@@ -296,18 +296,19 @@ template <typename T, int THREADS, int NV> struct Held {
         for (int g = 0; g < NV; g += G)
             if (s.v0 + g * THREADS < s.v1) step_vectors<T, THREADS, G, MASK>(s, s.v0 + g * THREADS, t, raw + g, f);
     }
-    // publish(largest logit) is called by every thread before the work-group meets for the maximum, met() right after
-    // (what it leaves in shared memory can be read when the sums are there).
-    template <bool ENTROPY, typename P, typename M>
+    // publish(largest logit) is called by every thread before the work-group meets for the maximum, met(maximum) right
+    // after (what it leaves in shared memory can be read when the sums are there).  EXTRA: dot is the work-group's sum of
+    // what met() returns.
+    template <bool ENTROPY, bool EXTRA, typename P, typename M>
     __device__ __forceinline__ RowSum sums(const Slice& s, uint32_t t, float c, float* red, P publish, M met) {
         RowSum r;
         const float single = LogitVec<T>::value(edge);
         r.top = single;
         steps<true>(s, t, [&](auto count, const u32x4* x, uint32_t) { r.top = fmaxf(r.top, largest_of<T, decltype(count)::value>(x)); });
         r.m = group_max<THREADS>(r.top, red, [&]() { publish(r.top); });
-        met();
-        r.sum = r.dot = 0.f;
         const float m = r.m == -kInf ? 0.f : r.m;
+        const float extra = met(m);
+        r.sum = r.dot = 0.f;
         if (!is_wide(m, c)) {
             const float mc = m * c, d = fmaf(m, c, -mc);   // d: what rounding left out of m c
             bool clamp = false;
@@ -325,7 +326,8 @@ template <typename T, int THREADS, int NV> struct Held {
             });
             add_term<ENTROPY>((single - m) * c, r.sum, r.dot);
         }
-        group_sum<THREADS, ENTROPY>(r.sum, r.dot, red);
+        if (EXTRA) r.dot = extra;
+        group_sum<THREADS, ENTROPY || EXTRA>(r.sum, r.dot, red);
         return r;
     }
 };
@@ -353,8 +355,10 @@ template <typename T, int THREADS> struct Streamed {
     }
     // early(f) is called once, by every thread, f() giving its largest logit among the first vectors; meet(count, vectors,
     // largest, base) for what every step holds.
-    template <bool ENTROPY, typename E, typename M>
-    static __device__ __forceinline__ RowSum sums(const RowSpan<T>& span, const Slice& s, uint32_t t, float c, float* red, E early, M meet) {
+    // EXTRA, met: as above.
+    template <bool ENTROPY, bool EXTRA, typename E, typename M, typename F>
+    static __device__ __forceinline__ RowSum sums(const RowSpan<T>& span, const Slice& s, uint32_t t, float c, float* red, E early, M meet,
+                                                  F met) {
         RowSum r;
         r.top = -kInf;
         r.sum = r.dot = 0.f;
@@ -388,14 +392,14 @@ template <typename T, int THREADS> struct Streamed {
             for (int g = 0; g < G; g += P)
                 if (base + g * THREADS < s.v1) step_vectors<T, THREADS, P, true>(s, base + g * THREADS, t, raw + g, step);
         };
-        if (s.v1 > s.v0) {   // (the second vectors are on their way while early() has the work-group meet)
+        if (s.v1 > s.v0) {
             u32x4 raw[2 * G];
             load_vectors<T, THREADS, 2 * G>(span, s, s.v0, t, raw);
             early([&]() {
                 float hi = LogitVec<T>::value(edge);
-                step_vectors<T, THREADS, G, true>(s, s.v0, t, raw, [&](auto count, const u32x4* x, uint32_t) {
-                    hi = fmaxf(hi, largest_of<T, decltype(count)::value>(x));
-                });
+                auto top = [&](auto count, const u32x4* x, uint32_t) { hi = fmaxf(hi, largest_of<T, decltype(count)::value>(x)); };
+                step_vectors<T, THREADS, G, true>(s, s.v0, t, raw, top);
+                if (s.v0 + G * THREADS < s.v1) step_vectors<T, THREADS, G, true>(s, s.v0 + G * THREADS, t, raw + G, top);
                 return hi;
             });
             steps(raw, s.v0);
@@ -426,7 +430,8 @@ template <typename T, int THREADS> struct Streamed {
             r.sum *= f;
         }
         r.m = top;
-        group_sum<THREADS, ENTROPY>(r.sum, r.dot, red);
+        if (EXTRA) r.dot = met(top == -kInf ? 0.f : top);
+        group_sum<THREADS, ENTROPY || EXTRA>(r.sum, r.dot, red);
         return r;
     }
 };
@@ -447,12 +452,14 @@ __device__ __forceinline__ uint64_t composite(uint32_t order, uint32_t index) { 
 // groups of threads are compared: the k-th largest of those is at most the slice's k-th largest logit, and hardly more
 // than k logits reach it (256 groups and k = 20: 21 expected), so only the threads whose own largest does look at their
 // vectors again.  A slice with more equal or clustered logits than the list holds takes the exact threshold instead.
-template <typename T, int THREADS> struct TopSelect {
-    static constexpr int LIST = 512;
+// HELD: vectors per thread, where that is all there are (0: more).
+template <typename T, int THREADS, int HELD> struct TopSelect {
     static constexpr int N = LogitVec<T>::N;
+    // (shared memory bounds how many short rows a compute unit works on at a time)
+    static constexpr int VECTORS = HELD && HELD * THREADS < 256 ? HELD * THREADS : 256;
+    static constexpr int LIST = HELD && HELD * THREADS * N + 16 < 512 ? HELD * THREADS * N + 16 : 512;
     static constexpr int GROUPS = THREADS < 256 ? THREADS : 256;
     static constexpr int LOW_BIT = sizeof(T) == 2 ? 16 : 0;   // bf16 logits are told apart by the upper half
-    static constexpr int VECTORS = 256;
     struct Shared {
         u32x4 vectors[VECTORS];       // vectors that hold a logit above the threshold
         uint64_t list[LIST];          // composites
@@ -671,7 +678,12 @@ template <int THREADS, typename F> __device__ __forceinline__ void ranked(const 
         const uint32_t i = i0 + threadIdx.x / share, part = threadIdx.x % share;
         const uint64_t mine = i < n ? list[i] : ~0ull;
         int rank = 0;
-        for (uint32_t j = part; j < n; j += share) rank += list[j] > mine;
+        uint32_t j = part;   // (four reads in flight)
+        for (; j + 3 * share < n; j += 4 * share) {
+            const uint64_t a = list[j], b = list[j + share], c = list[j + 2 * share], d = list[j + 3 * share];
+            rank += (a > mine) + (b > mine) + (c > mine) + (d > mine);
+        }
+        for (; j < n; j += share) rank += list[j] > mine;
         if (share > 1) rank += __builtin_amdgcn_update_dpp(0, rank, 0xB1, 0xf, 0xf, true);
         if (share > 2) rank += __builtin_amdgcn_update_dpp(0, rank, 0x4E, 0xf, 0xf, true);
         if (share > 4) rank += __builtin_amdgcn_update_dpp(0, rank, 0x141, 0xf, 0xf, true);
@@ -728,7 +740,6 @@ template <typename T, int THREADS> struct NamedLogits {
 };
 
 template <bool ENTROPY> __device__ __forceinline__ void write_row_sums(const LogprobParams& p, size_t row, const RowSum& r, float l) {
-    if (threadIdx.x != 0) return;
     if (p.stats) { p.stats[2 * row] = r.m; p.stats[2 * row + 1] = l; }
     if (ENTROPY) {
         const float h = (l - r.dot / r.sum) * kLn2;
@@ -736,72 +747,301 @@ template <bool ENTROPY> __device__ __forceinline__ void write_row_sums(const Log
     }
 }
 
-// One work-group per row, held in registers (NV vectors per thread) or, NV = 0, streamed.
+template <int THREADS> __device__ __forceinline__ void write_alternatives(const LogprobParams& p, size_t row, const uint64_t* list,
+                                                                        uint32_t n, const RowSum& r, float l) {
+    ranked<THREADS>(list, n, p.top_k, [&](uint32_t rank, uint64_t c) {
+        p.top_ids[row * p.top_k + rank] = (int32_t)~(uint32_t)c;
+        p.top_logprobs[row * p.top_k + rank] = log_prob(logit_of((uint32_t)(c >> 32)), r.m, l, p.scale);
+    });
+}
+
+// Short rows: one work-group per row, held in registers (NV vectors per thread).
 template <typename T, int THREADS, int NV, bool ENTROPY>
-__global__ __launch_bounds__(THREADS, NV == 0 ? 8 : 4) void token_logprobs_kernel(LogprobParams p) {
-    typedef TopSelect<T, THREADS> Top;
-    __shared__ float red[32];
+__global__ __launch_bounds__(THREADS) void token_logprobs_held_kernel(LogprobParams p) {
+    typedef TopSelect<T, THREADS, NV> Top;
+    __shared__ float red[2 * THREADS / 64];
     constexpr int N = LogitVec<T>::N;
-    const uint32_t t = threadIdx.x;
+    const uint32_t t = threadIdx.x, k = p.top_k;
     const size_t row = blockIdx.x;
     const RowSpan<T> span((const T*)p.logits + row * p.stride, p.vocab);
     const Slice s = slice_of(span, p.vocab, 0, 1, 0, t);
     NamedLogits<T, THREADS> named;
     named.load_ids(p.tokens + row * p.n_tokens, p.n_tokens);
-    const uint32_t k = p.top_k;
-    typedef Held<T, THREADS, NV ? NV : 1> Registers;
-    typedef Streamed<T, THREADS> Stream;
-    Registers held;
-    RowSum r;
+    Held<T, THREADS, NV> held;
+    held.load(span, s, t);
+    named.load_logits(span, p.vocab);
     const bool any = t < s.v1 || s.edge >= 0;
-    float least = __builtin_nanf("");
-    if (NV) {
-        held.load(span, s, t);
-        named.load_logits(span, p.vocab);
-        auto publish = [&](float hi) { if (k) Top::publish(hi, any, k); };
-        auto met = [&]() { if (k) Top::find(k); };
-        r = held.template sums<ENTROPY>(s, t, p.c, red, publish, met);
-    } else {
-        named.load_logits(span, p.vocab);
-        auto early = [&](auto first) { if (k) least = Top::early(first(), any, k); };
-        auto meet = [&](auto count, const u32x4* raw, float hi, uint32_t base) {
-            Top::template meet<decltype(count)::value>(span, raw, hi, base, least);
-        };
-        r = Stream::template sums<ENTROPY>(span, s, t, p.c, red, early, meet);
-    }
+    auto publish = [&](float hi) { if (k) Top::publish(hi, any, k); };
+    auto met = [&](float) {
+        if (k) Top::find(k);
+        return 0.f;
+    };
+    const RowSum r = held.template sums<ENTROPY, false>(s, t, p.c, red, publish, met);
     const float l = log2f(r.sum);
-    write_row_sums<ENTROPY>(p, row, r, l);
+    if (t == 0) write_row_sums<ENTROPY>(p, row, r, l);
     named.write(p.logprob + row * p.n_tokens, p.n_tokens, r.m, l, p.scale);
     if (k == 0) return;
+    if (THREADS == 64) __syncthreads();
+    bool exact;
+    const uint32_t limit = Top::found(&exact);
+    auto look = [&](float from) {
+        held.template steps<false>(s, t, [&](auto count, const u32x4* raw, uint32_t base) {
+            Top::template meet<decltype(count)::value>(span, raw, largest_of<T, decltype(count)::value>(raw), base, from);
+        });
+    };
+    auto every = [&](float from) {
+        held.each(s, t, [&](const float (&x)[N], uint32_t base) { Top::scan(x, span.index(base + t), from); });
+    };
+    Top::select(span, s, limit, exact, r.top, r.sum != r.sum, k, look, every);
+    write_alternatives<THREADS>(p, row, Top::shared().list, Top::shared().count, r, l);
+}
+
+// The sums of a streamed slice; with k > 0 its logits from `least` on are collected on the way.
+template <typename T, int THREADS, bool ENTROPY>
+__device__ __forceinline__ RowSum sum_and_collect(const RowSpan<T>& span, const Slice& s, float c, float* red, uint32_t k, bool any,
+                                                  float& least) {
+    typedef TopSelect<T, THREADS, 0> Top;
+    least = __builtin_nanf("");
+    auto early = [&](auto first) { if (k) least = Top::early(first(), any, k); };
+    auto meet = [&](auto count, const u32x4* raw, float hi, uint32_t base) {
+        Top::template meet<decltype(count)::value>(span, raw, hi, base, least);
+    };
+    return Streamed<T, THREADS>::template sums<ENTROPY, false>(span, s, threadIdx.x, c, red, early, meet, [](float) { return 0.f; });
+}
+// At least the k largest in the list.  Where the early threshold let too many through, or none, the row is read again.
+template <typename T, int THREADS>
+__device__ __forceinline__ void finish_collection(const RowSpan<T>& span, const Slice& s, const RowSum& r, uint32_t k, bool any, float least) {
+    typedef TopSelect<T, THREADS, 0> Top;
+    constexpr int N = LogitVec<T>::N;
+    const uint32_t t = threadIdx.x;
     const bool nan = r.sum != r.sum;
+    if (least == least) Top::edge(span, s, least);
+    Top::sift(least);
+    if (least == least && !nan && !Top::overflow()) return;
     bool exact = false;
-    if (NV) {
-        if (THREADS == 64) __syncthreads();
-        const uint32_t limit = Top::found(&exact);
-        auto look = [&](float from) {
-            held.template steps<false>(s, t, [&](auto count, const u32x4* raw, uint32_t base) {
-                Top::template meet<decltype(count)::value>(span, raw, largest_of<T, decltype(count)::value>(raw), base, from);
-            });
-        };
-        auto every = [&](float from) {
-            held.each(s, t, [&](const float (&x)[N], uint32_t base) { Top::scan(x, span.index(base + t), from); });
-        };
-        Top::select(span, s, limit, exact, r.top, nan, k, look, every);
-    } else {
-        if (least == least) Top::edge(span, s, least);
-        Top::sift(least);
-        if (!(least == least) || nan || Top::overflow()) {
-            const uint32_t limit = nan ? 0u : Top::threshold(r.top, any, k, &exact);
-            auto every = [&](float from) {
-                Stream::each(span, s, t, [&](const float (&x)[N], uint32_t base) { Top::scan(x, span.index(base + t), from); });
-            };
-            Top::select(span, s, limit, exact, r.top, nan, k, every, every);
+    const uint32_t limit = nan ? 0u : Top::threshold(r.top, any, k, &exact);
+    auto every = [&](float from) {
+        Streamed<T, THREADS>::each(span, s, t, [&](const float (&x)[N], uint32_t base) { Top::scan(x, span.index(base + t), from); });
+    };
+    Top::select(span, s, limit, exact, r.top, nan, k, every, every);
+}
+
+// Long rows: one work-group per row, streamed.
+template <typename T, int THREADS, bool ENTROPY>
+__global__ __launch_bounds__(THREADS, 8) void token_logprobs_stream_kernel(LogprobParams p) {
+    typedef TopSelect<T, THREADS, 0> Top;
+    __shared__ float red[2 * THREADS / 64];
+    const uint32_t t = threadIdx.x, k = p.top_k;
+    const size_t row = blockIdx.x;
+    const RowSpan<T> span((const T*)p.logits + row * p.stride, p.vocab);
+    const Slice s = slice_of(span, p.vocab, 0, 1, 0, t);
+    NamedLogits<T, THREADS> named;
+    named.load_ids(p.tokens + row * p.n_tokens, p.n_tokens);
+    named.load_logits(span, p.vocab);
+    const bool any = t < s.v1 || s.edge >= 0;
+    float least;
+    const RowSum r = sum_and_collect<T, THREADS, ENTROPY>(span, s, p.c, red, k, any, least);
+    const float l = log2f(r.sum);
+    if (t == 0) write_row_sums<ENTROPY>(p, row, r, l);
+    named.write(p.logprob + row * p.n_tokens, p.n_tokens, r.m, l, p.scale);
+    if (k == 0) return;
+    finish_collection<T, THREADS>(span, s, r, k, any, least);
+    write_alternatives<THREADS>(p, row, Top::shared().list, Top::shared().count, r, l);
+}
+
+// Very short rows: 16 lanes a row, so that a wave's instructions serve four rows and every reduction is four DPP moves.
+// Up to kShortTop alternatives are taken out one by one.
+constexpr uint32_t kShortTop = 8, kShortVecs = 64, kShortRows = 16;
+
+template <int CTRL> __device__ __forceinline__ uint32_t dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+template <typename V, typename F> __device__ __forceinline__ V over16(V v, F f) {
+    v = f(v, dpp<0xB1>(v));
+    v = f(v, dpp<0x4E>(v));
+    v = f(v, dpp<0x141>(v));
+    return f(v, dpp<0x140>(v));
+}
+
+template <typename T, bool ENTROPY>
+__global__ __launch_bounds__(256) void token_logprobs_short_kernel(LogprobParams p, uint32_t rows) {
+    constexpr int N = LogitVec<T>::N, VECS = kShortVecs / 16, E = VECS * N + 1;
+    const uint32_t g = threadIdx.x & 15, wanted = blockIdx.x * kShortRows + threadIdx.x / 16;
+    const size_t row = wanted < rows ? wanted : rows - 1;   // (lanes past the last row repeat it and write nothing)
+    const bool writes = wanted < rows;
+    const RowSpan<T> span((const T*)p.logits + row * p.stride, p.vocab);
+    const int32_t edge = span.edge(g);
+    u32x4 raw[VECS];
+#pragma unroll
+    for (int u = 0; u < VECS; ++u) raw[u] = u32x4{LogitVec<T>::kMasked, LogitVec<T>::kMasked, LogitVec<T>::kMasked, LogitVec<T>::kMasked};
+    if (span.vecs > 0) {
+#pragma unroll
+        for (int u = 0; u < VECS; ++u) {
+            const uint32_t i = g + 16 * u;
+            raw[u] = __builtin_nontemporal_load(span.at(0, i < span.vecs ? i : span.vecs - 1));
         }
     }
-    ranked<THREADS>(Top::shared().list, Top::shared().count, k, [&](uint32_t rank, uint64_t c) {
-        p.top_ids[row * p.top_k + rank] = (int32_t)~(uint32_t)c;
-        p.top_logprobs[row * p.top_k + rank] = log_prob(logit_of((uint32_t)(c >> 32)), r.m, l, p.scale);
-    });
+    uint32_t edge_bits = LogitVec<T>::kMaskedOne;
+    if (edge >= 0) edge_bits = LogitVec<T>::bits(span.row + edge);
+    float x[E];
+#pragma unroll
+    for (int u = 0; u < VECS; ++u) {
+        if (g + 16 * u >= span.vecs) raw[u] = u32x4{LogitVec<T>::kMasked, LogitVec<T>::kMasked, LogitVec<T>::kMasked, LogitVec<T>::kMasked};
+        float v[N];
+        LogitVec<T>::unpack(raw[u], v);
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[u * N + j] = v[j];
+    }
+    x[E - 1] = LogitVec<T>::value(edge_bits);
+    RowSum r;
+    r.top = largest(x);
+    r.m = over16(r.top, [](float a, float b) { return fmaxf(a, b); });
+    r.sum = r.dot = 0.f;
+    const float m = r.m == -kInf ? 0.f : r.m;
+#pragma unroll
+    for (int e = 0; e < E; ++e) add_term<ENTROPY>((x[e] - m) * p.c, r.sum, r.dot);
+    const auto plus = [](float a, float b) { return a + b; };
+    r.sum = over16(r.sum, plus);
+    if (ENTROPY) r.dot = over16(r.dot, plus);
+    const float l = log2f(r.sum);
+    if (g == 0 && writes) write_row_sums<ENTROPY>(p, row, r, l);
+    for (uint32_t i = g; i < p.n_tokens; i += 16) {
+        const int32_t id = p.tokens[row * p.n_tokens + i];
+        float lp = 0.f;
+        if (id >= 0 && (uint32_t)id < p.vocab) lp = log_prob(LogitVec<T>::load(span.row + id), r.m, l, p.scale);
+        if (writes) p.logprob[row * p.n_tokens + i] = lp;
+    }
+    if (p.top_k == 0) return;
+    // an element that is not there is below every logit
+    uint32_t order[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const bool there = e == E - 1 ? edge >= 0 : g + 16 * (e / N) < span.vecs;
+        order[e] = there ? order_of(x[e]) : 0u;
+    }
+    for (uint32_t k = 0; k < p.top_k; ++k) {
+        uint32_t mine = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) mine = mine > order[e] ? mine : order[e];
+        const uint32_t best = over16(mine, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
+        uint32_t index = 0xffffffffu;   // the lowest one that has it
+#pragma unroll
+        for (int e = E - 1; e >= 0; --e) {
+            const uint32_t j = e == E - 1 ? (uint32_t)edge : span.index(g + 16 * (e / N)) + e % N;
+            if (order[e] == best && j < index) index = j;
+        }
+        index = over16(index, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const uint32_t j = e == E - 1 ? (uint32_t)edge : span.index(g + 16 * (e / N)) + e % N;
+            if (j == index) order[e] = 0;
+        }
+        if (g == 0 && writes) {
+            p.top_ids[row * p.top_k + k] = (int32_t)index;
+            p.top_logprobs[row * p.top_k + k] = log_prob(logit_of(best), r.m, l, p.scale);
+        }
+    }
+}
+
+// ---- few long rows --------------------------------------------------------------------------------------------
+// Each row is cut into parts with a work-group each.  A part leaves its sums and its own k largest in the workspace; the
+// one that arrives last joins them (in the order of the parts) and writes the row, and clears the row's counter.  Records
+// go through the memory system's coherent level with device-scope stores and loads; a part waits for its stores before
+// it counts itself as arrived.
+constexpr uint32_t kSplitRows = 256, kSplitParts = 64, kSplitThreads = 512;
+
+struct SplitWork {
+    uint32_t* counters;   // [kSplitRows], zero between launches
+    uint8_t* records;
+    uint32_t parts, each, record_bytes;
+};
+
+template <typename V> __device__ __forceinline__ void leave(V* p, V v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <typename V> __device__ __forceinline__ V take(const V* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+template <typename T, bool ENTROPY>
+__global__ __launch_bounds__(kSplitThreads, 8) void token_logprobs_split_kernel(LogprobParams p, SplitWork w) {
+    constexpr int THREADS = kSplitThreads;
+    typedef TopSelect<T, THREADS, 0> Top;
+    typedef Streamed<T, THREADS> Stream;
+    __shared__ float red[2 * THREADS / 64];
+    __shared__ uint32_t arrived;
+    __shared__ float joined[3];
+    const uint32_t t = threadIdx.x, k = p.top_k, part = blockIdx.x % w.parts;
+    const size_t row = blockIdx.x / w.parts;
+    const RowSpan<T> span((const T*)p.logits + row * p.stride, p.vocab);
+    const Slice s = slice_of(span, p.vocab, part, w.parts, w.each, t);
+    NamedLogits<T, THREADS> named;
+    named.load_ids(p.tokens + row * p.n_tokens, p.n_tokens);
+    named.load_logits(span, p.vocab);
+    const bool any = s.v0 + t < s.v1 || s.edge >= 0;
+    float least;
+    RowSum r = sum_and_collect<T, THREADS, ENTROPY>(span, s, p.c, red, k, any, least);
+    uint8_t* const records = w.records + row * w.parts * w.record_bytes;
+    uint8_t* const record = records + part * w.record_bytes;
+    if (t < 3) leave((float*)record + t, t == 0 ? r.m : t == 1 ? r.sum : r.dot);
+    if (k) {
+        finish_collection<T, THREADS>(span, s, r, k, any, least);
+        const uint32_t n = Top::shared().count;
+        uint64_t* const best = (uint64_t*)(record + 16);
+        ranked<THREADS>(Top::shared().list, n, k, [&](uint32_t rank, uint64_t c) { leave(best + rank, c); });
+        for (uint32_t i = n + t; i < k; i += THREADS) leave(best + i, (uint64_t)0);   // (a part of fewer logits)
+    }
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+    __syncthreads();
+    if (t == 0) arrived = __hip_atomic_fetch_add(w.counters + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (arrived != w.parts - 1) return;
+    if (t < 64) {
+        float m = -kInf, sum = 0.f, dot = 0.f;
+        if (t < w.parts) {
+            const float* const f = (const float*)(records + t * w.record_bytes);
+            m = take(f);
+            sum = take(f + 1);
+            dot = take(f + 2);
+        }
+        const float top = wave_max(m);
+        if (m != top) {   // from this part's reference to the row's
+            const float d = (m - top) * p.c, f = exp2_fast(d);
+            if (ENTROPY) dot = f * (dot + fmaxf(d, -256.f) * sum);
+            sum *= f;
+        }
+        sum = wave_sum(sum);
+        if (ENTROPY) dot = wave_sum(dot);
+        if (t == 0) {
+            joined[0] = top;
+            joined[1] = sum;
+            joined[2] = dot;
+            leave(w.counters + row, 0u);
+        }
+    }
+    if (k) {
+        // At least k of the parts' logits reach the least of their r-th largest ones, r parts >= k: with that as a
+        // threshold about two k of the parts k are ranked.
+        const uint32_t r = (k + w.parts - 1) / w.parts;
+        if (t == 0) Top::shared().count = 0;
+        if (t < 64) {
+            uint32_t order = 0xffffffffu;
+            if (t < w.parts) order = (uint32_t)(take((const uint64_t*)(records + t * w.record_bytes + 16) + r - 1) >> 32);
+            order = over16(order, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+            if (t % 16 == 0) Top::shared().words[t / 16] = order;
+        }
+        __syncthreads();
+        uint32_t limit = Top::shared().words[0];
+        for (int i = 1; i < 4; ++i) limit = limit < Top::shared().words[i] ? limit : Top::shared().words[i];
+        for (uint32_t i = t; i < w.parts * k; i += THREADS) {
+            const uint64_t c = take((const uint64_t*)(records + (i / k) * w.record_bytes + 16) + i % k);
+            if ((uint32_t)(c >> 32) >= limit) Top::append((uint32_t)(c >> 32), ~(uint32_t)c);
+        }
+    }
+    __syncthreads();
+    r.m = joined[0];
+    r.sum = joined[1];
+    r.dot = joined[2];
+    const float l = log2f(r.sum);
+    if (t == 0) write_row_sums<ENTROPY>(p, row, r, l);
+    named.write(p.logprob + row * p.n_tokens, p.n_tokens, r.m, l, p.scale);
+    if (k) write_alternatives<THREADS>(p, row, Top::shared().list, Top::shared().count, r, l);
 }
 
 // ---- gradients ------------------------------------------------------------------------------------------------
@@ -825,39 +1065,67 @@ struct RowGrad {
     }
 };
 
-// Writes a slice of a row's gradient, then the entries in it that tokens name.  Equal tokens add up in slot order and the
-// first of them writes the entry.  d may be the logits themselves: the named ones are read before anything is written.
-// ids, coef: shared memory, complete.  each(f): f(x, base) for every vector of the thread.
-template <typename T, int THREADS, bool ENTROPY, typename EACH>
-__device__ __forceinline__ void write_gradient(const RowSpan<T>& span, const Slice& s, T* d, const RowGrad& g, const int32_t* ids,
-                                               const float* coef, uint32_t n, float scale, EACH each) {
-    constexpr int N = LogitVec<T>::N;
-    constexpr uint32_t ROUNDS = THREADS < (int)kMaxSlots ? kMaxSlots / THREADS : 1;
-    const uint32_t t = threadIdx.x;
-    float named[ROUNDS];
-    bool writes[ROUNDS];
+// The tokens that a row's coefficients belong to, and those coefficients, in shared memory, filled up with id -1 to a
+// whole number of fours.
+struct Slots {
+    int32_t id[kMaxSlots];
+    float coef[kMaxSlots];
+};
+template <int THREADS> __device__ __forceinline__ void pad_slots(Slots& slots, uint32_t n) {
+    if (n + threadIdx.x < (n + 3) / 4 * 4) {   // (at most three)
+        slots.id[n + threadIdx.x] = -1;
+        slots.coef[n + threadIdx.x] = 0.f;
+    }
+}
+// The gradient's entries that tokens name: equal tokens add up in slot order, and the first of them writes the entry.
+template <typename T, int THREADS> struct NamedEntries {
+    static constexpr uint32_t ROUNDS = THREADS < (int)kMaxSlots ? kMaxSlots / THREADS : 1;
+    float value[ROUNDS];
+    int32_t id[ROUNDS];   // -1: nothing to write
+    // sums of the coefficients of this thread's tokens in elements [e0, e1)
+    __device__ __forceinline__ void total(const Slots& slots, uint32_t n, uint32_t e0, uint32_t e1) {
 #pragma unroll
-    for (uint32_t r = 0; r < ROUNDS; ++r) {
-        const uint32_t i = t + r * THREADS;
-        writes[r] = false;
-        named[r] = 0.f;
-        if (i < n) {
-            const int32_t id = ids[i];
-            if (id >= 0 && (uint32_t)id >= s.e0 && (uint32_t)id < s.e1) {
-                const float x = LogitVec<T>::load(span.row + id);
-                float total = 0.f;
-                bool first = true;
-                for (uint32_t k = 0; k < n; ++k)
-                    if (ids[k] == id) {
-                        if (k < i) { first = false; break; }
-                        total += coef[k];
-                    }
-                writes[r] = first;
-                named[r] = fmaf(scale, total, g.template at<ENTROPY>(x));
+        for (uint32_t r = 0; r < ROUNDS; ++r) {
+            const uint32_t i = threadIdx.x + r * THREADS;
+            id[r] = -1;
+            value[r] = 0.f;
+            if (i >= n) continue;
+            const int32_t mine = slots.id[i];
+            if (mine < 0 || (uint32_t)mine < e0 || (uint32_t)mine >= e1) continue;
+            float sum = 0.f;
+            bool first = true;
+#pragma unroll 2
+            for (uint32_t k = 0; k < n; k += 4) {
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) {
+                    const bool same = slots.id[k + j] == mine;
+                    sum += same ? slots.coef[k + j] : 0.f;
+                    first = first && !(same && k + j < i);
+                }
             }
+            if (first) id[r] = mine;
+            value[r] = sum;
         }
     }
-    __syncthreads();
+    // the rest of these entries: their own logits, read before any gradient is written (d may be the logits)
+    template <bool ENTROPY> __device__ __forceinline__ void finish(const RowSpan<T>& span, const RowGrad& g, float scale) {
+#pragma unroll
+        for (uint32_t r = 0; r < ROUNDS; ++r)
+            if (id[r] >= 0) value[r] = fmaf(scale, value[r], g.template at<ENTROPY>(LogitVec<T>::load(span.row + id[r])));
+    }
+    __device__ __forceinline__ void write(T* d) const {
+#pragma unroll
+        for (uint32_t r = 0; r < ROUNDS; ++r)
+            if (id[r] >= 0) LogitVec<T>::store(d + id[r], value[r]);
+    }
+};
+
+// Writes a slice of a row's gradient but for the entries that tokens name; d may be the logits themselves.  each(f):
+// f(x, base) for every vector of the thread.
+template <typename T, bool ENTROPY, typename EACH>
+__device__ __forceinline__ void write_gradient(const RowSpan<T>& span, const Slice& s, T* d, const RowGrad& g, EACH each) {
+    constexpr int N = LogitVec<T>::N;
+    const uint32_t t = threadIdx.x;
     const RowSpan<T> to = span.onto(d);
     each([&](float (&x)[N], uint32_t base) {
 #pragma unroll
@@ -865,10 +1133,6 @@ __device__ __forceinline__ void write_gradient(const RowSpan<T>& span, const Sli
         __builtin_nontemporal_store(LogitVec<T>::pack(x), (u32x4*)to.at(base, t));
     });
     if (s.edge >= 0) LogitVec<T>::store(d + s.edge, g.template at<ENTROPY>(LogitVec<T>::load(span.row + s.edge)));
-    __syncthreads();
-#pragma unroll
-    for (uint32_t r = 0; r < ROUNDS; ++r)
-        if (writes[r]) LogitVec<T>::store(d + ids[t + r * THREADS], named[r]);
 }
 
 // A row that nothing reaches (padding): zeros, whatever its logits hold.
@@ -880,51 +1144,59 @@ template <typename T, int THREADS> __device__ __forceinline__ void write_zeros(c
 }
 
 // ---- a teacher's list -----------------------------------------------------------------------------------------
-__device__ __forceinline__ float teacher_logit(const void* z, int as_bf16, size_t i) {
-    return as_bf16 ? bf16_bits_to_f32(((const uint16_t*)z)[i]) : ((const float*)z)[i];
-}
-
-// Softmax of a teacher's list over its used slots, by one wave: q[0 .. n); returns sum q log2 q.  *some: there is a
-// distribution (a used slot above -inf).
-__device__ __forceinline__ float teacher_softmax(const int32_t* ids, const void* z, int as_bf16, size_t first, uint32_t n,
-                                                 uint32_t vocab, float c, float* q, bool* some) {
-    const uint32_t lane = threadIdx.x & 63;
-    float v[kMaxSlots / 64], hi = -kInf;
+// One wave's view of a teacher's list: the softmax over its used slots.
+struct Teacher {
+    static constexpr uint32_t ROUNDS = kMaxSlots / 64;
+    uint32_t bits[ROUNDS];
+    float minus_entropy;   // sum q log2 q
+    bool some;             // there is a distribution: a used slot above -inf
+    __device__ __forceinline__ void load(const void* z, int as_bf16, size_t first, uint32_t n) {
 #pragma unroll
-    for (uint32_t r = 0; r < kMaxSlots / 64; ++r) {
-        const uint32_t i = lane + 64 * r;
-        v[r] = -kInf;
-        if (i < n) {
-            const float zi = teacher_logit(z, as_bf16, first + i);
-            const int32_t id = ids[first + i];
-            if (id >= 0 && (uint32_t)id < vocab) v[r] = zi;
+        for (uint32_t r = 0; r < ROUNDS; ++r) {
+            const uint32_t i = (threadIdx.x & 63) + 64 * r;
+            bits[r] = 0;
+            if (64 * r < n && i < n) bits[r] = as_bf16 ? ((const uint16_t*)z)[first + i] : ((const uint32_t*)z)[first + i];
         }
-        hi = fmaxf(hi, v[r]);
     }
-    hi = wave_max(hi);
-    float sum = 0.f;
+    // q[0 .. n) from the slots' ids; what is past n is left alone
+    __device__ __forceinline__ void softmax(const int32_t* ids, int as_bf16, uint32_t n, uint32_t vocab, float c, float* q) {
+        const uint32_t lane = threadIdx.x & 63;
+        float v[ROUNDS], hi = -kInf;
 #pragma unroll
-    for (uint32_t r = 0; r < kMaxSlots / 64; ++r)
-        if (v[r] != -kInf) sum += exp2_fast((v[r] - hi) * c);
-    sum = wave_sum(sum);
-    const float l = log2f(sum);
-    float minus_entropy = 0.f;
-#pragma unroll
-    for (uint32_t r = 0; r < kMaxSlots / 64; ++r) {
-        const uint32_t i = lane + 64 * r;
-        if (i < n) {
-            float qi = 0.f;
-            if (v[r] != -kInf) {
-                const float lq = (v[r] - hi) * c - l;
-                qi = exp2_fast(lq);
-                minus_entropy += qi * fmaxf(lq, -256.f);
+        for (uint32_t r = 0; r < ROUNDS; ++r) {
+            const uint32_t i = lane + 64 * r;
+            v[r] = -kInf;
+            if (i < n) {
+                const int32_t id = ids[i];
+                if (id >= 0 && (uint32_t)id < vocab) v[r] = as_bf16 ? bf16_bits_to_f32(bits[r]) : __builtin_bit_cast(float, bits[r]);
             }
-            q[i] = qi;
+            hi = fmaxf(hi, v[r]);
         }
+        hi = wave_max(hi);
+        float sum = 0.f;
+#pragma unroll
+        for (uint32_t r = 0; r < ROUNDS; ++r)
+            if (v[r] != -kInf) sum += exp2_fast((v[r] - hi) * c);
+        sum = wave_sum(sum);
+        const float l = log2f(sum);
+        minus_entropy = 0.f;
+#pragma unroll
+        for (uint32_t r = 0; r < ROUNDS; ++r) {
+            const uint32_t i = lane + 64 * r;
+            if (i < n) {
+                float qi = 0.f;
+                if (v[r] != -kInf) {
+                    const float lq = (v[r] - hi) * c - l;
+                    qi = exp2_fast(lq);
+                    minus_entropy += qi * fmaxf(lq, -256.f);
+                }
+                q[i] = qi;
+            }
+        }
+        some = !(sum == 0.f);
+        minus_entropy = wave_sum(minus_entropy);
     }
-    *some = !(sum == 0.f);
-    return wave_sum(minus_entropy);
-}
+};
 
 // ---- gradients from a row's statistics ------------------------------------------------------------------------
 struct GradParams {
@@ -942,15 +1214,11 @@ struct GradParams {
     float scale, c;
 };
 
-constexpr int kGradThreads = 256, kGradVecs = 4;
-
-// One work-group per kGradThreads * kGradVecs vectors of a row.
-template <typename T, bool ENTROPY, bool TEACHER>
-__global__ __launch_bounds__(kGradThreads) void logit_gradient_kernel(GradParams p) {
-    constexpr int THREADS = kGradThreads;
+// One work-group per THREADS * NV vectors of a row.
+template <typename T, int THREADS, int NV, bool ENTROPY, bool TEACHER>
+__global__ __launch_bounds__(THREADS) void logit_gradient_kernel(GradParams p) {
     __shared__ float red[2 * THREADS / 64];
-    __shared__ float coef[kMaxSlots];
-    __shared__ int32_t ids[kMaxSlots];
+    __shared__ Slots slots;
     __shared__ uint32_t some_teacher;
     const uint32_t t = threadIdx.x;
     const size_t row = blockIdx.x / p.parts;
@@ -959,43 +1227,60 @@ __global__ __launch_bounds__(kGradThreads) void logit_gradient_kernel(GradParams
     T* const d = (T*)p.d_logits + row * p.stride;
     const float m = p.stats[2 * row], l = p.stats[2 * row + 1];
     const float ent = ENTROPY ? -p.scale * p.d_entropy[row] : 0.f, H = ENTROPY ? p.entropy[row] : 0.f;
-    float C = 0.f, any = 0.f;
+    const float w = TEACHER ? p.d_loss[row] / (p.scale * p.scale) : 0.f;
+    if (l == -kInf || (TEACHER && w == 0.f)) {
+        write_zeros<T, THREADS>(span, s, d);
+        return;
+    }
+    Held<T, THREADS, NV> held;
+    NamedEntries<T, THREADS> named;
+    float C = 0.f;
     if (TEACHER) {
-        const float w = p.d_loss[row] / (p.scale * p.scale);
-        if (t < 64) {
-            bool some;
-            teacher_softmax(p.ids, p.teacher, p.teacher_bf16, row * p.n, p.n, p.vocab, p.c, coef, &some);
-            if (t == 0) some_teacher = some ? 1u : 0u;
-        }
+        Teacher teacher;
+        if (t < 64) teacher.load(p.teacher, p.teacher_bf16, row * p.n, p.n);
+        for (uint32_t i = t; i < p.n; i += THREADS) slots.id[i] = p.ids[row * p.n + i];
+        held.load(span, s, t);
         __syncthreads();
-        for (uint32_t i = t; i < p.n; i += THREADS) {
-            ids[i] = p.ids[row * p.n + i];
-            coef[i] *= -w;
+        if (t < 64) {
+            teacher.softmax(slots.id, p.teacher_bf16, p.n, p.vocab, p.c, slots.coef);
+            if (t == 0) some_teacher = teacher.some ? 1u : 0u;
+        }
+        pad_slots<THREADS>(slots, p.n);
+        __syncthreads();
+        if (!some_teacher) {
+            write_zeros<T, THREADS>(span, s, d);
+            return;
         }
         C = -w;
-        any = some_teacher ? w : 0.f;
+        named.total(slots, p.n, s.e0, s.e1);
+#pragma unroll
+        for (uint32_t r = 0; r < named.ROUNDS; ++r) named.value[r] *= -w;
     } else {
+        float any = 0.f;
         for (uint32_t i = t; i < p.n; i += THREADS) {
             const int32_t id = p.ids[row * p.n + i];
             const float v = p.d_logprob[row * p.n + i];
             const bool inside = id >= 0 && (uint32_t)id < p.vocab;
-            ids[i] = id;
-            coef[i] = inside ? v : 0.f;
+            slots.id[i] = id;
+            slots.coef[i] = inside ? v : 0.f;
             if (inside) { C += v; any += v != 0.f ? 1.f : 0.f; }
         }
-        group_sum<THREADS, true>(C, any, red);
-        if (ent != 0.f) any = 1.f;
+        pad_slots<THREADS>(slots, p.n);
+        group_sum<THREADS, true>(C, any, red);   // (its barriers complete the slots too)
+        if (any == 0.f && ent == 0.f) {
+            write_zeros<T, THREADS>(span, s, d);
+            return;
+        }
+        held.load(span, s, t);
+        named.total(slots, p.n, s.e0, s.e1);
     }
-    if (any == 0.f || l == -kInf) {
-        write_zeros<T, THREADS>(span, s, d);
-        return;
-    }
-    Held<T, THREADS, kGradVecs> held;
-    held.load(span, s, t);
     RowGrad g;
     g.set(m, l, p.c, -p.scale * C, ent, H);
-    __syncthreads();   // ids and coef are complete
-    write_gradient<T, THREADS, ENTROPY>(span, s, d, g, ids, coef, p.n, p.scale, [&](auto f) { held.each(s, t, f); });
+    named.template finish<ENTROPY>(span, g, p.scale);
+    __syncthreads();
+    write_gradient<T, ENTROPY>(span, s, d, g, [&](auto f) { held.each(s, t, f); });
+    __syncthreads();
+    named.write(d);
 }
 
 // ---- distillation ---------------------------------------------------------------------------------------------
@@ -1012,38 +1297,32 @@ struct DistillParams {
     float scale, c;
 };
 
-// Loss over a teacher's slots from the student's statistics, by one wave: q [n] in shared memory, *some as above.
-template <typename T>
-__device__ __forceinline__ float teacher_loss(const DistillParams& p, size_t row, const RowSpan<T>& span, float m, float l, float* q,
-                                              bool* some) {
-    const float minus_entropy = teacher_softmax(p.ids, p.teacher, p.teacher_bf16, row * p.n, p.n, p.vocab, p.c, q, some);
-    float cross = 0.f;
-    for (uint32_t i = threadIdx.x & 63; i < p.n; i += 64)
-        if (!(q[i] <= 0.f)) cross += q[i] * log_prob(LogitVec<T>::load(span.row + p.ids[row * p.n + i]), m, l, p.scale);
-    cross = wave_sum(cross);
-    return *some ? (minus_entropy * kLn2 - cross) / (p.scale * p.scale) : 0.f;
-}
-
 // One work-group per row, held in registers (NV vectors per thread) or, NV = 0, streamed: the student's sums, the loss,
-// and (GRAD) the gradient, for which a held row is not read again.
+// and (GRAD) the gradient, for which a held row is not read again.  The teacher's softmax and the logits of its tokens
+// are ready by the time the row has arrived; with m, l of the student and q of the teacher the loss is
+//   ( sum q ln q - sum q (x - m) s + ln2 l ) / s^2.
 template <typename T, int THREADS, int NV, bool GRAD>
 __global__ __launch_bounds__(THREADS, THREADS == 1024 && NV == 8 ? 8 : 4) void distill_kernel(DistillParams p) {
-    __shared__ float red[32];
-    __shared__ float q[kMaxSlots];
-    __shared__ int32_t ids[kMaxSlots];
+    __shared__ float red[2 * THREADS / 64];
+    __shared__ Slots slots;
     __shared__ uint32_t some_teacher;
     const uint32_t t = threadIdx.x;
     const size_t row = blockIdx.x;
     const RowSpan<T> span((const T*)p.logits + row * p.stride, p.vocab);
     const Slice s = slice_of(span, p.vocab, 0, 1, 0, t);
     T* const d = GRAD ? (T*)p.d_logits + row * p.stride : nullptr;
+    NamedLogits<T, THREADS> logits;
+    Teacher teacher;
+    if (t < 64) teacher.load(p.teacher, p.teacher_bf16, row * p.n, p.n);
+    logits.load_ids(p.ids + row * p.n, p.n);
     float used = 0.f;
-    for (uint32_t i = t; i < p.n; i += THREADS) {
-        const int32_t id = p.ids[row * p.n + i];
-        ids[i] = id;
-        if (id >= 0 && (uint32_t)id < p.vocab) used = 1.f;
+#pragma unroll
+    for (int r = 0; r < logits.ROUNDS; ++r) {
+        const uint32_t i = t + r * THREADS;
+        if (i < p.n) slots.id[i] = logits.id[r];
+        if ((uint32_t)logits.id[r] < p.vocab) used = 1.f;
     }
-    used = group_max<THREADS>(used, red, []() {});
+    used = group_max<THREADS>(used, red, [&]() { pad_slots<THREADS>(slots, p.n); });
     if (used == 0.f) {   // no slot (padding): the logits are not read
         if (t == 0) {
             p.row_loss[row] = 0.f;
@@ -1052,61 +1331,94 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 && NV == 8 ? 8 : 4) void d
         if (GRAD) write_zeros<T, THREADS>(span, s, d);
         return;
     }
+    logits.load_logits(span, p.vocab);
+    NamedEntries<T, THREADS> named;
+    // (called when the maximum is known: q is complete)
+    auto met = [&](float m) {
+        float cross = 0.f;
+#pragma unroll
+        for (int r = 0; r < logits.ROUNDS; ++r) {
+            const uint32_t i = t + r * THREADS;
+            const float q = i < p.n ? slots.coef[i] : 0.f;
+            if (!(q <= 0.f)) cross += q * ((LogitVec<T>::value(logits.x[r]) - m) * p.scale);
+        }
+        if (GRAD) named.total(slots, p.n, 0, p.vocab);
+        return cross;
+    };
+    auto softmax = [&]() {
+        if (t >= 64) return;
+        teacher.softmax(slots.id, p.teacher_bf16, p.n, p.vocab, p.c, slots.coef);
+        if (t == 0) some_teacher = teacher.some ? 1u : 0u;
+    };
     Held<T, THREADS, NV ? NV : 1> held;
     RowSum r;
     if (NV) {
         held.load(span, s, t);
-        r = held.template sums<false>(s, t, p.c, red, [](float) {}, []() {});
+        softmax();
+        r = held.template sums<false, true>(s, t, p.c, red, [](float) {}, met);
     } else {
-        r = Streamed<T, THREADS>::template sums<false>(span, s, t, p.c, red, [](auto) {}, [](auto, const u32x4*, float, uint32_t) {});
+        softmax();
+        r = Streamed<T, THREADS>::template sums<false, true>(span, s, t, p.c, red, [](auto) {}, [](auto, const u32x4*, float, uint32_t) {}, met);
     }
     const float l = log2f(r.sum);
-    if (t < 64) {
-        bool some;
-        const float loss = teacher_loss<T>(p, row, span, r.m, l, q, &some);
-        if (t == 0) {
-            p.row_loss[row] = loss;
-            if (p.stats) { p.stats[2 * row] = r.m; p.stats[2 * row + 1] = l; }
-            some_teacher = some ? 1u : 0u;
-        }
+    const bool some = some_teacher != 0;
+    if (t == 0) {
+        // (no logit above -inf: the student gives the teacher's tokens no probability)
+        const float loss = l == -kInf ? kInf : (teacher.minus_entropy + l) * kLn2 - r.dot;
+        p.row_loss[row] = some ? loss / (p.scale * p.scale) : 0.f;
+        if (p.stats) { p.stats[2 * row] = r.m; p.stats[2 * row + 1] = l; }
     }
-    if (GRAD) {
-        const float w = p.d_loss[row] / (p.scale * p.scale);
-        __syncthreads();
-        if (!some_teacher || w == 0.f || l == -kInf) {
-            write_zeros<T, THREADS>(span, s, d);
-            return;
-        }
-        for (uint32_t i = t; i < p.n; i += THREADS) q[i] *= -w;
-        __syncthreads();
-        RowGrad g;
-        g.set(r.m, l, p.c, p.scale * w, 0.f, 0.f);
-        write_gradient<T, THREADS, false>(span, s, d, g, ids, q, p.n, p.scale, [&](auto f) {
-            if (NV) held.each(s, t, f);
-            else Streamed<T, THREADS>::each(span, s, t, f);
-        });
+    if (!GRAD) return;
+    const float w = p.d_loss[row] / (p.scale * p.scale);
+    if (!some || w == 0.f || l == -kInf) {
+        write_zeros<T, THREADS>(span, s, d);
+        return;
     }
+    RowGrad g;
+    g.set(r.m, l, p.c, p.scale * w, 0.f, 0.f);
+#pragma unroll
+    for (uint32_t i = 0; i < named.ROUNDS; ++i)
+        if (named.id[i] >= 0) named.value[i] = fmaf(-p.scale * w, named.value[i], g.template at<false>(LogitVec<T>::value(logits.x[i])));
+    if (!NV) __syncthreads();   // (a streamed row is read again, its named logits have been)
+    write_gradient<T, false>(span, s, d, g, [&](auto f) {
+        if (NV) held.each(s, t, f);
+        else Streamed<T, THREADS>::each(span, s, t, f);
+    });
+    __syncthreads();
+    named.write(d);
 }
 
 // How a row is spread over a work-group: threads, and vectors per thread held in registers (0: streamed).
 struct RowShape { int threads, vecs; };
-static inline RowShape logprobs_shape(uint32_t vocab, int dtype) {
+static inline RowShape distill_shape(uint32_t vocab, int dtype, bool gradient) {
     const uint32_t vecs = vocab / (dtype == SFB_BF16 ? 8u : 4u);
     if (vecs <= 64) return {64, 1};
     if (vecs <= 256) return {64, 4};
     if (vecs <= 1024) return {256, 4};
-    return {512, 0};
-}
-static inline RowShape distill_shape(uint32_t vocab, int dtype) {
-    const uint32_t vecs = vocab / (dtype == SFB_BF16 ? 8u : 4u);
-    if (vecs <= 64) return {64, 1};
-    if (vecs <= 256) return {64, 4};
-    if (vecs <= 1024) return {256, 4};
+    if (!gradient) return {512, 0};
     if (vecs <= 2048) return {256, 8};
     if (vecs <= 4096) return {512, 8};
     if (vecs <= 8192) return {1024, 8};
     if (vecs <= 16384) return {1024, 16};
     return {1024, 0};
+}
+
+// Parts of each row of a launch that would otherwise leave most of the device idle; 1: rows stay whole.
+static inline SplitWork split_rows(void* workspace, uint64_t rows, uint32_t vecs, uint32_t k) {
+    SplitWork w{};
+    w.parts = 1;
+    if (!workspace || rows > kSplitRows || vecs < 2048) return w;
+    uint32_t parts = 768 / (uint32_t)rows;
+    if (parts > vecs / 1024) parts = vecs / 1024;
+    if (parts > kSplitParts) parts = kSplitParts;
+    if (k && parts > 512 / k) parts = 512 / k;   // (the parts' alternatives fit one list)
+    if (parts < 2) return w;
+    w.parts = parts;
+    w.each = (vecs + parts - 1) / parts;
+    w.record_bytes = 16 + (k * 8 + 15) / 16 * 16;
+    w.counters = (uint32_t*)workspace;
+    w.records = (uint8_t*)workspace + kSplitRows * sizeof(uint32_t);
+    return w;
 }
 
 static inline int check_logits(const void* logits, int dtype, uint64_t rows, uint32_t vocab, uint64_t stride, float scale,
@@ -1143,14 +1455,20 @@ extern "C" int sfb_token_logprobs(sfb_stream_t stream, float* logprob, float* en
                     scale * kLog2e};
     hipStream_t s = (hipStream_t)stream;
     clear_stale_error();
-    const RowShape shape = logprobs_shape(vocab, dtype);
+    const uint32_t vecs = vocab / (dtype == SFB_BF16 ? 8u : 4u);
+    const SplitWork w = split_rows(workspace, rows, vecs, top_k);
     const dim3 grid((uint32_t)rows);
-#define SFB_LP_AS(T, ENT)                                                                                        \
-    do {                                                                                                         \
-        if (shape.threads == 64 && shape.vecs == 1) token_logprobs_kernel<T, 64, 1, ENT><<<grid, 64, 0, s>>>(p); \
-        else if (shape.threads == 64) token_logprobs_kernel<T, 64, 4, ENT><<<grid, 64, 0, s>>>(p);               \
-        else if (shape.threads == 256) token_logprobs_kernel<T, 256, 4, ENT><<<grid, 256, 0, s>>>(p);            \
-        else token_logprobs_kernel<T, 512, 0, ENT><<<grid, 512, 0, s>>>(p);                                      \
+#define SFB_LP_AS(T, ENT)                                                                                              \
+    do {                                                                                                               \
+        if (w.parts > 1)                                                                                               \
+            token_logprobs_split_kernel<T, ENT><<<dim3((uint32_t)rows * w.parts), kSplitThreads, 0, s>>>(p, w);        \
+        else if (vecs <= kShortVecs && top_k <= kShortTop)                                                             \
+            token_logprobs_short_kernel<T, ENT><<<dim3((uint32_t)((rows + kShortRows - 1) / kShortRows)), 256, 0, s>>>(p, (uint32_t)rows); \
+        else if (vecs <= 64) token_logprobs_held_kernel<T, 64, 1, ENT><<<grid, 64, 0, s>>>(p);                         \
+        else if (vecs <= 256) token_logprobs_held_kernel<T, 64, 4, ENT><<<grid, 64, 0, s>>>(p);                        \
+        else if (vecs <= 1024) token_logprobs_held_kernel<T, 256, 4, ENT><<<grid, 256, 0, s>>>(p);                     \
+        else if (top_k && vecs <= 4096) token_logprobs_stream_kernel<T, 256, ENT><<<grid, 256, 0, s>>>(p);             \
+        else token_logprobs_stream_kernel<T, 512, ENT><<<grid, 512, 0, s>>>(p);                                        \
     } while (0)
 #define SFB_LP(T)                        \
     do {                                 \
@@ -1166,20 +1484,20 @@ extern "C" int sfb_token_logprobs(sfb_stream_t stream, float* logprob, float* en
 
 static int launch_gradient(hipStream_t s, GradParams& p, int dtype, uint64_t rows, bool entropy, bool teacher) {
     const uint32_t vecs = p.vocab / (dtype == SFB_BF16 ? 8u : 4u);
-    p.each = kGradThreads * kGradVecs;
+    p.each = teacher ? 512 * 8 : 256 * 4;
     p.parts = vecs == 0 ? 1 : (vecs + p.each - 1) / p.each;
     if (rows * p.parts > 0x7fffffffull) return SFB_ERR_SHAPE;
     const dim3 grid((uint32_t)(rows * p.parts));
     clear_stale_error();
-    if (dtype == SFB_F32) {
-        if (teacher) logit_gradient_kernel<float, false, true><<<grid, kGradThreads, 0, s>>>(p);
-        else if (entropy) logit_gradient_kernel<float, true, false><<<grid, kGradThreads, 0, s>>>(p);
-        else logit_gradient_kernel<float, false, false><<<grid, kGradThreads, 0, s>>>(p);
-    } else {
-        if (teacher) logit_gradient_kernel<__bf16, false, true><<<grid, kGradThreads, 0, s>>>(p);
-        else if (entropy) logit_gradient_kernel<__bf16, true, false><<<grid, kGradThreads, 0, s>>>(p);
-        else logit_gradient_kernel<__bf16, false, false><<<grid, kGradThreads, 0, s>>>(p);
-    }
+#define SFB_GR(T)                                                                                       \
+    do {                                                                                                \
+        if (teacher) logit_gradient_kernel<T, 512, 8, false, true><<<grid, 512, 0, s>>>(p);             \
+        else if (entropy) logit_gradient_kernel<T, 256, 4, true, false><<<grid, 256, 0, s>>>(p);        \
+        else logit_gradient_kernel<T, 256, 4, false, false><<<grid, 256, 0, s>>>(p);                    \
+    } while (0)
+    if (dtype == SFB_F32) SFB_GR(float);
+    else SFB_GR(__bf16);
+#undef SFB_GR
     return launch_status();
 }
 
@@ -1217,18 +1535,19 @@ extern "C" int sfb_distillation_loss(sfb_stream_t stream, float* row_loss, float
                     teacher_dtype == SFB_BF16 ? 1 : 0, scale, scale * kLog2e};
     hipStream_t s = (hipStream_t)stream;
     clear_stale_error();
-    const RowShape shape = distill_shape(vocab, dtype);
+    const RowShape shape = distill_shape(vocab, dtype, d_logits != nullptr);
     const dim3 grid((uint32_t)rows);
 #define SFB_DL_AS(T, GRAD)                                                                                         \
     do {                                                                                                           \
         if (shape.threads == 64 && shape.vecs == 1) distill_kernel<T, 64, 1, GRAD><<<grid, 64, 0, s>>>(p);         \
         else if (shape.threads == 64) distill_kernel<T, 64, 4, GRAD><<<grid, 64, 0, s>>>(p);                       \
         else if (shape.threads == 256 && shape.vecs == 4) distill_kernel<T, 256, 4, GRAD><<<grid, 256, 0, s>>>(p); \
-        else if (shape.threads == 256) distill_kernel<T, 256, 8, GRAD><<<grid, 256, 0, s>>>(p);                    \
-        else if (shape.threads == 512) distill_kernel<T, 512, 8, GRAD><<<grid, 512, 0, s>>>(p);                    \
-        else if (shape.vecs == 8) distill_kernel<T, 1024, 8, GRAD><<<grid, 1024, 0, s>>>(p);                       \
-        else if (shape.vecs == 16) distill_kernel<T, 1024, 16, GRAD><<<grid, 1024, 0, s>>>(p);                     \
-        else distill_kernel<T, 1024, 0, GRAD><<<grid, 1024, 0, s>>>(p);                                            \
+        else if (!GRAD) distill_kernel<T, 512, 0, false><<<grid, 512, 0, s>>>(p);                                  \
+        else if (shape.threads == 256) distill_kernel<T, 256, 8, true><<<grid, 256, 0, s>>>(p);                    \
+        else if (shape.threads == 512) distill_kernel<T, 512, 8, true><<<grid, 512, 0, s>>>(p);                    \
+        else if (shape.vecs == 8) distill_kernel<T, 1024, 8, true><<<grid, 1024, 0, s>>>(p);                       \
+        else if (shape.vecs == 16) distill_kernel<T, 1024, 16, true><<<grid, 1024, 0, s>>>(p);                     \
+        else distill_kernel<T, 1024, 0, true><<<grid, 1024, 0, s>>>(p);                                            \
     } while (0)
 #define SFB_DL(T)                         \
     do {                                  \

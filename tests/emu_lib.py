@@ -461,7 +461,7 @@ def load(tag="", defines=()):
         else:
             os.environ["SFBERT_HIP_LIB"] = saved
     mod._stream = lambda: None
-    mod._require_device = lambda *tensors: None
+    mod._stream_for = lambda *tensors: None
     mod.to_device = lambda a: tensor(np.ascontiguousarray(a).view(np.uint8).reshape(-1))
     lib = mod.lib
     lib.emu_guarded_alloc.restype = C.c_void_p
