@@ -3,6 +3,7 @@ alternatives, and the distillation loss against a teacher's top logits, each wit
 
 ``own`` False: the operators in elementary torch operations (fp32, rounded once at the end); True: the calls that a user
 makes of the package."""
+import functools
 import math
 
 import torch
@@ -189,7 +190,8 @@ def _plain_distill(s):
 
 
 # ---------------------------------------------------------------------------------------------- the package
-def _package():
+@functools.lru_cache(maxsize=None)
+def _package():   # a program imports it once
     import importlib
     return importlib.import_module("sf-bert_amd")
 
