@@ -652,6 +652,7 @@ int sfb_softmax_cross_entropy(sfb_stream_t stream, float* loss, float* row_loss,
  * do not depend on the order in which threads run: the same inputs give the same bits.
  * stats [dev] float[rows][2] (may be NULL): the row's reference logit m and log2 sum_j 2^((x_j - m) scale log2(e)),
  * which the backward entry points take; with s = scale, ln sum_j exp(s x_j) = s m + ln(2) stats[1].
+ * rows x the threads of a row (64 to 1024) stay below 2^32, or the call returns SFB_ERR_SHAPE.
  * workspace [dev] 16-byte aligned, SFB_LOGIT_WORKSPACE_BYTES bytes, zero-filled once before its first use and left
  * ready for the next launch, or NULL: with it, few long rows are each cut over several work-groups.  Launches that
  * share a workspace must be ordered on one stream (graphs captured with one are replayed one after the other). */

@@ -972,7 +972,9 @@ def _logit_workspace(workspace):
 def _tokens(tokens, rows):
     """(pointer, tokens per row) of int32 [rows] or [rows, n]"""
     import torch
-    n = 1 if tokens.dim() == 1 else tokens.shape[-1]
+    if tokens.dim() not in (1, 2):
+        raise SfbError(4, "tokens of %d dimensions" % tokens.dim())
+    n = 1 if tokens.dim() == 1 else tokens.shape[1]
     return _small(tokens, (rows,) if tokens.dim() == 1 else (rows, n), torch.int32, "tokens"), n
 
 
@@ -1034,7 +1036,9 @@ def token_logprobs_backward(logits, tokens, stats, d_logprob=None, entropy=None,
 
 def _teacher(teacher_ids, teacher_logits, rows):
     import torch
-    slots = teacher_ids.shape[-1]
+    if teacher_ids.dim() != 2:
+        raise SfbError(4, "teacher_ids of %d dimensions" % teacher_ids.dim())
+    slots = teacher_ids.shape[1]
     return (_small(teacher_ids, (rows, slots), torch.int32, "teacher_ids"),
             _small(teacher_logits, (rows, slots), teacher_logits.dtype, "teacher_logits"), _dtype_code(teacher_logits), slots)
 

@@ -948,16 +948,54 @@ __global__ __launch_bounds__(256) void token_logprobs_short_kernel(LogprobParams
 // one that arrives last joins them (in the order of the parts) and writes the row, and clears the row's counter.  Records
 // go through the memory system's coherent level with device-scope stores and loads; a part waits for its stores before
 // it counts itself as arrived.
-constexpr uint32_t kSplitRows = 256, kSplitParts = 64, kSplitThreads = 512;
+constexpr uint32_t kSplitRows = 512, kSplitParts = 64, kSplitThreads = 512, kSplitGroups = 1024;
 
 struct SplitWork {
     uint32_t* counters;   // [kSplitRows], zero between launches
+    float* stats;         // [kSplitRows][2], where the caller keeps none
     uint8_t* records;
     uint32_t parts, each, record_bytes;
 };
 
 template <typename V> __device__ __forceinline__ void leave(V* p, V v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 template <typename V> __device__ __forceinline__ V take(const V* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
+// Counts this part of `row` as arrived, once all that the work-group has left is there; whether it is the last.
+__device__ __forceinline__ bool arrive(const SplitWork& w, size_t row, uint32_t* arrived) {
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) *arrived = __hip_atomic_fetch_add(w.counters + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    return *arrived == w.parts - 1;
+}
+// The row's sums from its parts' ones (m, sum, dot at the start of each record), by one wave, in joined[0 .. 3); clears the
+// row's counter.
+template <bool ENTROPY>
+__device__ __forceinline__ void join_sums(const SplitWork& w, size_t row, const uint8_t* records, float c, float* joined) {
+    const uint32_t t = threadIdx.x;
+    if (t >= 64) return;
+    float m = -kInf, sum = 0.f, dot = 0.f;
+    if (t < w.parts) {
+        const float* const f = (const float*)(records + t * w.record_bytes);
+        m = take(f);
+        sum = take(f + 1);
+        if (ENTROPY) dot = take(f + 2);
+    }
+    const float top = wave_max(m);
+    if (m != top) {   // from this part's reference to the row's
+        const float d = (m - top) * c, f = exp2_fast(d);
+        if (ENTROPY) dot = f * (dot + fmaxf(d, -256.f) * sum);
+        sum *= f;
+    }
+    sum = wave_sum(sum);
+    if (ENTROPY) dot = wave_sum(dot);
+    if (t == 0) {
+        joined[0] = top;
+        joined[1] = sum;
+        joined[2] = dot;
+        leave(w.counters + row, 0u);
+    }
+}
 
 template <typename T, bool ENTROPY>
 __global__ __launch_bounds__(kSplitThreads, 8) void token_logprobs_split_kernel(LogprobParams p, SplitWork w) {
@@ -987,34 +1025,8 @@ __global__ __launch_bounds__(kSplitThreads, 8) void token_logprobs_split_kernel(
         ranked<THREADS>(Top::shared().list, n, k, [&](uint32_t rank, uint64_t c) { leave(best + rank, c); });
         for (uint32_t i = n + t; i < k; i += THREADS) leave(best + i, (uint64_t)0);   // (a part of fewer logits)
     }
-    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");
-    __syncthreads();
-    if (t == 0) arrived = __hip_atomic_fetch_add(w.counters + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __syncthreads();
-    if (arrived != w.parts - 1) return;
-    if (t < 64) {
-        float m = -kInf, sum = 0.f, dot = 0.f;
-        if (t < w.parts) {
-            const float* const f = (const float*)(records + t * w.record_bytes);
-            m = take(f);
-            sum = take(f + 1);
-            dot = take(f + 2);
-        }
-        const float top = wave_max(m);
-        if (m != top) {   // from this part's reference to the row's
-            const float d = (m - top) * p.c, f = exp2_fast(d);
-            if (ENTROPY) dot = f * (dot + fmaxf(d, -256.f) * sum);
-            sum *= f;
-        }
-        sum = wave_sum(sum);
-        if (ENTROPY) dot = wave_sum(dot);
-        if (t == 0) {
-            joined[0] = top;
-            joined[1] = sum;
-            joined[2] = dot;
-            leave(w.counters + row, 0u);
-        }
-    }
+    if (!arrive(w, row, &arrived)) return;
+    join_sums<ENTROPY>(w, row, records, p.c, joined);
     if (k) {
         // At least k of the parts' logits reach the least of their r-th largest ones, r parts >= k: with that as a
         // threshold about two k of the parts k are ranked.
@@ -1214,9 +1226,13 @@ struct GradParams {
     float scale, c;
 };
 
-// One work-group per THREADS * NV vectors of a row.
-template <typename T, int THREADS, int NV, bool ENTROPY, bool TEACHER>
-__global__ __launch_bounds__(THREADS) void logit_gradient_kernel(GradParams p) {
+constexpr int kGradThreads = 256, kGradVecs = 4;
+constexpr uint32_t kSplitGradient = 8192;   // vectors up to which a row's loss and gradient stay one launch
+
+// One work-group per kGradThreads * kGradVecs vectors of a row.
+template <typename T, bool ENTROPY, bool TEACHER>
+__global__ __launch_bounds__(kGradThreads) void logit_gradient_kernel(GradParams p) {
+    constexpr int THREADS = kGradThreads, NV = kGradVecs;
     __shared__ float red[2 * THREADS / 64];
     __shared__ Slots slots;
     __shared__ uint32_t some_teacher;
@@ -1297,6 +1313,12 @@ struct DistillParams {
     float scale, c;
 };
 
+// cross: sum q (x - m) s.  (No logit above -inf: the student gives the teacher's tokens no probability.)
+__device__ __forceinline__ float row_loss(const Teacher& teacher, float l, float cross, float scale) {
+    const float loss = l == -kInf ? kInf : (teacher.minus_entropy + l) * kLn2 - cross;
+    return loss / (scale * scale);
+}
+
 // One work-group per row, held in registers (NV vectors per thread) or, NV = 0, streamed: the student's sums, the loss,
 // and (GRAD) the gradient, for which a held row is not read again.  The teacher's softmax and the logits of its tokens
 // are ready by the time the row has arrived; with m, l of the student and q of the teacher the loss is
@@ -1363,9 +1385,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 && NV == 8 ? 8 : 4) void d
     const float l = log2f(r.sum);
     const bool some = some_teacher != 0;
     if (t == 0) {
-        // (no logit above -inf: the student gives the teacher's tokens no probability)
-        const float loss = l == -kInf ? kInf : (teacher.minus_entropy + l) * kLn2 - r.dot;
-        p.row_loss[row] = some ? loss / (p.scale * p.scale) : 0.f;
+        p.row_loss[row] = some ? row_loss(teacher, l, r.dot, p.scale) : 0.f;
         if (p.stats) { p.stats[2 * row] = r.m; p.stats[2 * row + 1] = l; }
     }
     if (!GRAD) return;
@@ -1388,6 +1408,53 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 && NV == 8 ? 8 : 4) void d
     named.write(d);
 }
 
+// Few long rows: the sums and the loss, each row cut over several work-groups.
+template <typename T> __global__ __launch_bounds__(kSplitThreads, 8) void distill_split_kernel(DistillParams p, SplitWork w) {
+    constexpr int THREADS = kSplitThreads;
+    __shared__ float red[2 * THREADS / 64];
+    __shared__ Slots slots;
+    __shared__ uint32_t arrived;
+    __shared__ float joined[3];
+    const uint32_t t = threadIdx.x, part = blockIdx.x % w.parts;
+    const size_t row = blockIdx.x / w.parts;
+    const RowSpan<T> span((const T*)p.logits + row * p.stride, p.vocab);
+    const Slice s = slice_of(span, p.vocab, part, w.parts, w.each, t);
+    NamedLogits<T, THREADS> logits;
+    Teacher teacher;
+    if (t < 64) teacher.load(p.teacher, p.teacher_bf16, row * p.n, p.n);
+    logits.load_ids(p.ids + row * p.n, p.n);
+    float used = 0.f;
+    if (t < p.n) slots.id[t] = logits.id[0];
+    if ((uint32_t)logits.id[0] < p.vocab) used = 1.f;
+    used = group_max<THREADS>(used, red, []() {});
+    if (used == 0.f) {
+        if (t == 0 && part == 0) {
+            p.row_loss[row] = 0.f;
+            p.stats[2 * row] = p.stats[2 * row + 1] = -kInf;
+        }
+        return;
+    }
+    logits.load_logits(span, p.vocab);
+    RowSum r = Streamed<T, THREADS>::template sums<false, false>(span, s, t, p.c, red, [](auto) {}, [](auto, const u32x4*, float, uint32_t) {},
+                                                                [](float) { return 0.f; });
+    uint8_t* const records = w.records + row * w.parts * w.record_bytes;
+    if (t < 2) leave((float*)(records + part * w.record_bytes) + t, t == 0 ? r.m : r.sum);
+    if (!arrive(w, row, &arrived)) return;
+    join_sums<false>(w, row, records, p.c, joined);
+    if (t < 64) teacher.softmax(slots.id, p.teacher_bf16, p.n, p.vocab, p.c, slots.coef);
+    __syncthreads();
+    const float m = joined[0], l = log2f(joined[1]);
+    const float q = t < p.n ? slots.coef[t] : 0.f;
+    float cross = 0.f, unused = 0.f;
+    if (!(q <= 0.f)) cross = q * ((LogitVec<T>::value(logits.x[0]) - (m == -kInf ? 0.f : m)) * p.scale);
+    group_sum<THREADS, false>(cross, unused, red);
+    if (t == 0) {
+        p.row_loss[row] = teacher.some ? row_loss(teacher, l, cross, p.scale) : 0.f;
+        p.stats[2 * row] = m;
+        p.stats[2 * row + 1] = l;
+    }
+}
+
 // How a row is spread over a work-group: threads, and vectors per thread held in registers (0: streamed).
 struct RowShape { int threads, vecs; };
 static inline RowShape distill_shape(uint32_t vocab, int dtype, bool gradient) {
@@ -1408,7 +1475,7 @@ static inline SplitWork split_rows(void* workspace, uint64_t rows, uint32_t vecs
     SplitWork w{};
     w.parts = 1;
     if (!workspace || rows > kSplitRows || vecs < 2048) return w;
-    uint32_t parts = 768 / (uint32_t)rows;
+    uint32_t parts = kSplitGroups / (uint32_t)rows;
     if (parts > vecs / 1024) parts = vecs / 1024;
     if (parts > kSplitParts) parts = kSplitParts;
     if (k && parts > 512 / k) parts = 512 / k;   // (the parts' alternatives fit one list)
@@ -1417,7 +1484,8 @@ static inline SplitWork split_rows(void* workspace, uint64_t rows, uint32_t vecs
     w.each = (vecs + parts - 1) / parts;
     w.record_bytes = 16 + (k * 8 + 15) / 16 * 16;
     w.counters = (uint32_t*)workspace;
-    w.records = (uint8_t*)workspace + kSplitRows * sizeof(uint32_t);
+    w.stats = (float*)workspace + kSplitRows;
+    w.records = (uint8_t*)workspace + 3 * kSplitRows * sizeof(uint32_t);
     return w;
 }
 
@@ -1432,6 +1500,8 @@ static inline int check_logits(const void* logits, int dtype, uint64_t rows, uin
     if (workspace && workspace_bytes < SFB_LOGIT_WORKSPACE_BYTES) return SFB_ERR_WORKSPACE;
     return SFB_OK;
 }
+// A launch has fewer than 2^32 threads.
+static inline bool too_many(uint64_t groups, uint32_t threads) { return groups * threads > 0xffffffffull; }
 static inline bool misaligned4(const void* a, const void* b = nullptr, const void* c = nullptr, const void* d = nullptr) {
     return (((uintptr_t)a | (uintptr_t)b | (uintptr_t)c | (uintptr_t)d) & 3u) != 0;
 }
@@ -1457,12 +1527,14 @@ extern "C" int sfb_token_logprobs(sfb_stream_t stream, float* logprob, float* en
     clear_stale_error();
     const uint32_t vecs = vocab / (dtype == SFB_BF16 ? 8u : 4u);
     const SplitWork w = split_rows(workspace, rows, vecs, top_k);
+    const bool is_short = vecs <= kShortVecs && top_k <= kShortTop;
+    if (too_many(rows, is_short ? 256 / kShortRows : vecs <= 256 ? 64 : vecs <= 1024 ? 256 : 512)) return SFB_ERR_SHAPE;
     const dim3 grid((uint32_t)rows);
 #define SFB_LP_AS(T, ENT)                                                                                              \
     do {                                                                                                               \
         if (w.parts > 1)                                                                                               \
             token_logprobs_split_kernel<T, ENT><<<dim3((uint32_t)rows * w.parts), kSplitThreads, 0, s>>>(p, w);        \
-        else if (vecs <= kShortVecs && top_k <= kShortTop)                                                             \
+        else if (is_short)                                                                                             \
             token_logprobs_short_kernel<T, ENT><<<dim3((uint32_t)((rows + kShortRows - 1) / kShortRows)), 256, 0, s>>>(p, (uint32_t)rows); \
         else if (vecs <= 64) token_logprobs_held_kernel<T, 64, 1, ENT><<<grid, 64, 0, s>>>(p);                         \
         else if (vecs <= 256) token_logprobs_held_kernel<T, 64, 4, ENT><<<grid, 64, 0, s>>>(p);                        \
@@ -1484,16 +1556,16 @@ extern "C" int sfb_token_logprobs(sfb_stream_t stream, float* logprob, float* en
 
 static int launch_gradient(hipStream_t s, GradParams& p, int dtype, uint64_t rows, bool entropy, bool teacher) {
     const uint32_t vecs = p.vocab / (dtype == SFB_BF16 ? 8u : 4u);
-    p.each = teacher ? 512 * 8 : 256 * 4;
+    p.each = kGradThreads * kGradVecs;
     p.parts = vecs == 0 ? 1 : (vecs + p.each - 1) / p.each;
-    if (rows * p.parts > 0x7fffffffull) return SFB_ERR_SHAPE;
+    if (too_many(rows * p.parts, kGradThreads)) return SFB_ERR_SHAPE;
     const dim3 grid((uint32_t)(rows * p.parts));
     clear_stale_error();
 #define SFB_GR(T)                                                                                       \
     do {                                                                                                \
-        if (teacher) logit_gradient_kernel<T, 512, 8, false, true><<<grid, 512, 0, s>>>(p);             \
-        else if (entropy) logit_gradient_kernel<T, 256, 4, true, false><<<grid, 256, 0, s>>>(p);        \
-        else logit_gradient_kernel<T, 256, 4, false, false><<<grid, 256, 0, s>>>(p);                    \
+        if (teacher) logit_gradient_kernel<T, false, true><<<grid, kGradThreads, 0, s>>>(p);             \
+        else if (entropy) logit_gradient_kernel<T, true, false><<<grid, kGradThreads, 0, s>>>(p);        \
+        else logit_gradient_kernel<T, false, false><<<grid, kGradThreads, 0, s>>>(p);                    \
     } while (0)
     if (dtype == SFB_F32) SFB_GR(float);
     else SFB_GR(__bf16);
@@ -1535,7 +1607,23 @@ extern "C" int sfb_distillation_loss(sfb_stream_t stream, float* row_loss, float
                     teacher_dtype == SFB_BF16 ? 1 : 0, scale, scale * kLog2e};
     hipStream_t s = (hipStream_t)stream;
     clear_stale_error();
+    const uint32_t vecs = vocab / (dtype == SFB_BF16 ? 8u : 4u);
+    const SplitWork w = split_rows(d_logits && vecs <= kSplitGradient ? nullptr : workspace, rows, vecs, 0);
+    if (w.parts > 1) {   // the loss, then the gradient from the rows' statistics
+        if (!stats) p.stats = w.stats;
+        const dim3 parts((uint32_t)rows * w.parts);
+        if (dtype == SFB_F32) distill_split_kernel<float><<<parts, kSplitThreads, 0, s>>>(p, w);
+        else distill_split_kernel<__bf16><<<parts, kSplitThreads, 0, s>>>(p, w);
+        const int status = launch_status();
+        if (status || !d_logits) return status;
+        GradParams g{};
+        g.logits = logits; g.d_logits = d_logits; g.ids = teacher_ids; g.stats = p.stats; g.teacher = teacher_logits;
+        g.teacher_bf16 = p.teacher_bf16; g.d_loss = d_loss; g.stride = row_stride; g.vocab = vocab; g.n = slots;
+        g.scale = scale; g.c = p.c;
+        return launch_gradient(s, g, dtype, rows, false, true);
+    }
     const RowShape shape = distill_shape(vocab, dtype, d_logits != nullptr);
+    if (too_many(rows, (uint32_t)shape.threads)) return SFB_ERR_SHAPE;
     const dim3 grid((uint32_t)rows);
 #define SFB_DL_AS(T, GRAD)                                                                                         \
     do {                                                                                                           \

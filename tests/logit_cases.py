@@ -331,6 +331,31 @@ def teacher_to_student(S, dev, vocab=700, rows=6, slots=12, scale=0.5):
     assert abs((up - down) / (2 * step) - (d * direction).sum()) < 1e-5
 
 
+def parts_left_out(S, dev):
+    """Every combination of what a call can be asked for; the entropy's gradient alone."""
+    x = matrix(300, 3, False, KINDS[:6])
+    rows = x.shape[0]
+    t, tok = dev(x), dev(np.arange(rows, dtype=np.int32))
+    whole = S.token_logprobs(t, tok, top_k=3, entropy=True)
+    for tokens in (None, tok, tok.reshape(rows, 1)):
+        for k in (0, 3):
+            for entropy in (False, True):
+                got = S.token_logprobs(t, tokens, top_k=k, entropy=entropy)
+                assert set(got) == {"stats"} | ({"logprob"} if tokens is not None else set()) | \
+                    ({"top_ids", "top_logprobs"} if k else set()) | ({"entropy"} if entropy else set())
+                for name in got:
+                    assert np.array_equal(host(got[name]).reshape(-1), host(whole[name]).reshape(-1)), name
+                if tokens is not None:
+                    assert got["logprob"].shape == tokens.shape
+    ge = np.linspace(-1, 1, rows).astype(np.float32)
+    d = S.token_logprobs_backward(t, None, whole["stats"], entropy=whole["entropy"], d_entropy=dev(ge))
+    lp = plain_log_softmax(x, 1.0)
+    want = plain_gradient(x, lp, np.full((rows, 1), -1), np.zeros((rows, 1)), ge, 1.0)
+    with np.errstate(all="ignore"):
+        weight = np.abs(ge) * (20 + 2 * np.nan_to_num(plain_entropy(lp)))
+    same(host(d), want, gradient_tol(x, 1.0, lp, weight, want, False), "entropy's gradient")
+
+
 def refusals(S, dev):
     """Calls that are turned away, with the status that says why."""
     import pytest
@@ -355,6 +380,11 @@ def refusals(S, dev):
     turned_away("shape", lambda: S.token_logprobs(x, top_k=41))                     # more than the vocabulary
     turned_away("shape", lambda: S.token_logprobs(dev(np.zeros((1, 100), np.float32)), top_k=65))
     turned_away("shape", lambda: S.token_logprobs(x, dev(np.zeros((3, 257), np.int32))))
+    turned_away("shape", lambda: S.token_logprobs(x, tok.reshape(3, 1, 1)))
+    turned_away("shape", lambda: S.token_logprobs(x, tok[0]))
+    turned_away("shape", lambda: S.token_logprobs(x, top_k=-1))
+    turned_away("shape", lambda: S.distillation_loss(x, ids[0], z[0]))
+    turned_away("shape", lambda: S.token_logprobs_backward(x, tok, stats, d_logprob=row[:2]))
     turned_away("dtype", lambda: S.token_logprobs(x.double(), tok))
     turned_away("dtype", lambda: S.token_logprobs(x, tok.long()))
     turned_away("align", lambda: S.token_logprobs(x[:, 1:], tok))                   # first element off 16 bytes

@@ -69,13 +69,152 @@ def test_few_long_rows_cut_over_the_device(vocab, bf16, pad):
         cases.logprobs(S, dev, vocab, bf16, pad, n=n, k=k, workspace=ws, repeat=3, seed=20 + k)
         for kind in ("normal", "masked", "nan"):   # one row: the most parts
             cases.logprobs(S, dev, vocab, bf16, pad, n=n, k=k, workspace=ws, kinds=[kind], seed=40 + k)
+    for slots, teacher_bf16, in_place in ((1, False, False), (37, True, True), (256, False, False)):
+        cases.distillation(S, dev, vocab, bf16, pad, slots=slots, teacher_bf16=teacher_bf16, in_place=in_place, workspace=ws, seed=30 + slots)
     torch.cuda.synchronize()
-    assert int(ws[:1024].view(torch.int32).abs().sum()) == 0, "arrival counters must be left at zero"
+    assert int(ws[:2048].view(torch.int32).abs().sum()) == 0, "arrival counters must be left at zero"
 
 
 @pytest.mark.gpu
 def test_teacher_to_student_on_the_device():
     cases.teacher_to_student(*device_backend())
+
+
+@pytest.mark.gpu
+def test_parts_left_out_on_the_device():
+    cases.parts_left_out(*device_backend())
+
+
+@pytest.mark.gpu
+@pytest.mark.needs_device
+def test_host_tensors_are_refused():
+    S, dev = device_backend()
+    x = dev(np.zeros((2, 40), np.float32))
+    tok = torch.zeros(2, dtype=torch.int32)
+    for call in (lambda: S.token_logprobs(x, tok), lambda: S.token_logprobs(x.cpu(), tok), lambda: S.distillation_loss(x, tok[:, None], x[:, :1].cpu())):
+        with pytest.raises(S.SfbError) as e:
+            call()
+        assert e.value.status == 8
+
+
+@pytest.mark.gpu
+@pytest.mark.needs_device
+def test_on_another_stream():
+    S, dev = device_backend()
+    x = dev(cases.matrix(30522, 3, False, ["normal"] * 40))
+    tok = torch.arange(40, dtype=torch.int32, device="cuda")
+    want = S.token_logprobs(x, tok, top_k=8, entropy=True)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        got = S.token_logprobs(x, tok, top_k=8, entropy=True)
+        d = S.token_logprobs_backward(x, tok, got["stats"], d_logprob=got["logprob"])
+    side.synchronize()
+    for name in want:
+        assert torch.equal(got[name], want[name]), name
+    assert torch.equal(d, S.token_logprobs_backward(x, tok, want["stats"], d_logprob=want["logprob"]))
+
+
+@pytest.mark.gpu
+@pytest.mark.needs_device
+def test_captured_and_replayed_with_a_shared_workspace():
+    """Two graphs with one workspace, replayed in turn on changing inputs with eager calls between: every replay gives
+    what the eager call gives."""
+    S, dev = device_backend()
+    ws = torch.zeros(S.LOGIT_WORKSPACE_BYTES, dtype=torch.uint8, device="cuda")
+    rng = np.random.default_rng(5)
+    few, many = torch.empty((3, 70001), device="cuda"), torch.empty((900, 5003), device="cuda", dtype=torch.bfloat16)
+    tok = dev(rng.integers(0, 5003, 900).astype(np.int32))
+    ids, z = dev(rng.integers(0, 5003, (900, 17)).astype(np.int32)), dev(rng.standard_normal((900, 17)).astype(np.float32))
+    w = dev(rng.standard_normal(900).astype(np.float32))
+
+    def first():
+        a = S.token_logprobs(few, tok[:3], top_k=20, entropy=True, workspace=ws)
+        b = S.distillation_loss(few, ids[:3], z[:3], scale=0.5, d_loss=w[:3], workspace=ws)
+        return [a[n] for n in sorted(a)] + [b[n] for n in sorted(b)]
+
+    def second():
+        a = S.token_logprobs(many, tok, top_k=5, entropy=True, workspace=ws)
+        d = S.token_logprobs_backward(many, tok, a["stats"], d_logprob=w, entropy=a["entropy"], d_entropy=w)
+        b = S.distillation_loss(many, ids, z, scale=0.5, d_loss=w, workspace=ws)
+        c = S.distillation_loss(few, ids[:3], z[:3], workspace=ws)
+        return [a[n] for n in sorted(a)] + [b[n] for n in sorted(b)] + [c["row_loss"], d]
+
+    few.normal_()
+    many.normal_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        first(), second()
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for call in (first, second):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = call()
+        graphs.append((g, out, call))
+    for turn in range(4):
+        few.normal_(0, 1 + turn)
+        many.normal_(0, 1 + turn)
+        for g, out, call in graphs:
+            g.replay()
+            torch.cuda.synchronize()
+            for got, want in zip(out, call()):
+                assert torch.equal(got, want)
+    assert int(ws[:2048].view(torch.int32).abs().sum()) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.needs_device
+def test_offsets_past_32_bits():
+    """Rows that begin more than 2^32 elements (and 2^33 bytes) into the logits."""
+    S, _ = device_backend()
+    rows, vocab = 70000, 65541
+    x = torch.empty((rows, vocab), device="cuda", dtype=torch.bfloat16)
+    x.zero_()
+    x[-3:].normal_(0, 2)
+    x[0].normal_(0, 2)
+    tok = torch.full((rows,), 65540, device="cuda", dtype=torch.int32)
+    some = torch.tensor([0, rows - 3, rows - 2, rows - 1], device="cuda")
+    got = S.token_logprobs(x, tok, entropy=True)
+    lp = torch.log_softmax(x[some].double(), 1)
+    assert (got["logprob"][some].double() - lp[:, -1]).abs().max() < 2e-5
+    assert abs(float(got["logprob"][5]) + np.log(vocab)) < 2e-5 and abs(float(got["entropy"][5]) - np.log(vocab)) < 2e-4
+    g = torch.zeros(rows, device="cuda")
+    g[some] = 1.0
+    d = S.token_logprobs_backward(x, tok, got["stats"], d_logprob=g, out=x)
+    want = -lp.exp()
+    want[:, -1] += 1
+    assert (d[some].double() - want).abs().max() < 2.0 ** -8 * 1.01
+    assert not d[1:rows - 3:9999].any()
+    assert int((d[1:rows - 3] != 0).sum()) == 0
+
+
+@pytest.mark.gpu
+def test_model_scores_its_input():
+    """Model.score: the log probabilities of given tokens are minus the losses the model's own cross-entropy gives; the
+    best alternatives are its largest logits."""
+    S, dev = device_backend()
+    rng = np.random.default_rng(9)
+    bs, nb, heads, d, vocab, ffn = 64, 4, 2, 64, 500, 128
+    n, L = heads * d, bs * nb
+    f32 = lambda *shape: dev((rng.standard_normal(shape) * 0.05).astype(np.float32))   # noqa: E731
+    w = {name: f32(*shape) for name, shape in (("wq", (n, n)), ("wk", (n, n)), ("wv", (n, n)), ("wo", (n, n)), ("w1", (n, ffn)), ("w2", (ffn, n)),
+                                               ("bq", (n,)), ("bk", (n,)), ("bv", (n,)), ("bo", (n,)), ("b1", (ffn,)), ("b2", (n,)),
+                                               ("ln1_b", (n,)), ("ln2_b", (n,)))}
+    w["ln1_g"], w["ln2_g"] = (dev(np.ones(n, np.float32)) for _ in range(2))
+    model = S.Model(f32(vocab, n), f32(L, n), [w], S.build_luts(S.layout_local(nb, 1, bidirectional=True)), bs, heads, d, ffn)
+    ids = dev(rng.integers(0, vocab, (2, L)).astype(np.int32))
+    labels = dev(rng.integers(0, vocab, (2, L)).astype(np.int32))
+    logits = model.forward(ids, want_logits=True)["logits"]
+    _, row_loss = S.softmax_cross_entropy(logits, labels.reshape(-1))
+    got = model.score(ids, labels, top_k=10, entropy=True)
+    assert np.abs(cases.host(got["logprob"]) + cases.host(row_loss)).max() < 1e-5
+    assert np.array_equal(cases.host(got["top_ids"]), cases.plain_top(cases.host(logits).astype(np.float32), 10))
+    pair = torch.stack([labels, ids], dim=2).contiguous()
+    assert torch.equal(model.score(ids, pair)["logprob"][:, 0], got["logprob"])
+    with pytest.raises(S.SfbError):
+        model.score(ids, labels[:1])
 
 
 @pytest.mark.gpu
@@ -108,7 +247,8 @@ def test_few_long_rows_cut_on_the_host_model(E, vocab, bf16, order):   # noqa: F
     ws = dev(np.zeros(S.LOGIT_WORKSPACE_BYTES, np.uint8))
     cases.logprobs(S, dev, vocab, bf16, 3, n=5, k=9, workspace=ws, kinds=["normal", "masked", "rising", "nan", "all lowest", "empty"], repeat=2)
     cases.logprobs(S, dev, vocab, bf16, 0, n=1, k=64, workspace=ws, kinds=["ties"], seed=8)
-    assert not ws[:1024].any(), "arrival counters must be left at zero"
+    cases.distillation(S, dev, vocab, bf16, 0, slots=37, workspace=ws, kinds=["normal", "masked", "rising", "empty", "nan", "late peak"], in_place=True)
+    assert not ws[:2048].any(), "arrival counters must be left at zero"
 
 
 @pytest.mark.parametrize("order", [1, 14, 21])
@@ -122,6 +262,10 @@ def test_logit_ops_with_lanes_in_adverse_orders(E, order):   # noqa: F811
 
 def test_teacher_to_student_on_the_host_model(E):   # noqa: F811
     cases.teacher_to_student(*host_backend(E))
+
+
+def test_parts_left_out_on_the_host_model(E):   # noqa: F811
+    cases.parts_left_out(*host_backend(E))
 
 
 def test_refusals_on_the_host_model(E):   # noqa: F811
