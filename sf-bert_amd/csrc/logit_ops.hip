@@ -948,7 +948,7 @@ __global__ __launch_bounds__(256) void token_logprobs_short_kernel(LogprobParams
 // one that arrives last joins them (in the order of the parts) and writes the row, and clears the row's counter.  Records
 // go through the memory system's coherent level with device-scope stores and loads; a part waits for its stores before
 // it counts itself as arrived.
-constexpr uint32_t kSplitRows = 512, kSplitParts = 64, kSplitThreads = 512, kSplitGroups = 1024;
+constexpr uint32_t kSplitRows = 512, kSplitParts = 64, kSplitThreads = 512;
 
 struct SplitWork {
     uint32_t* counters;   // [kSplitRows], zero between launches
@@ -1466,20 +1466,22 @@ static inline RowShape distill_shape(uint32_t vocab, int dtype, bool gradient) {
     if (vecs <= 2048) return {256, 8};
     if (vecs <= 4096) return {512, 8};
     if (vecs <= 8192) return {1024, 8};
+    if (vecs <= 12288) return {1024, 12};
     if (vecs <= 16384) return {1024, 16};
     return {1024, 0};
 }
 
-// Parts of each row of a launch that would otherwise leave most of the device idle; 1: rows stay whole.
-static inline SplitWork split_rows(void* workspace, uint64_t rows, uint32_t vecs, uint32_t k) {
+// Parts of each row of a launch that would otherwise leave most of the device idle: about `groups` work-groups in all, of
+// at least 1024 vectors each.  (48 rows of 16384 vectors with 20 alternatives: 13 us as 240 groups, 15 as 480, 17 as 768,
+// 27 whole.)  parts = 0: no workspace, or too many rows.
+static inline SplitWork split_rows(void* workspace, uint64_t rows, uint32_t vecs, uint32_t k, uint32_t groups) {
     SplitWork w{};
-    w.parts = 1;
-    if (!workspace || rows > kSplitRows || vecs < 2048) return w;
-    uint32_t parts = kSplitGroups / (uint32_t)rows;
+    if (!workspace || rows > kSplitRows) return w;
+    uint32_t parts = groups / (uint32_t)rows;
     if (parts > vecs / 1024) parts = vecs / 1024;
     if (parts > kSplitParts) parts = kSplitParts;
     if (k && parts > 512 / k) parts = 512 / k;   // (the parts' alternatives fit one list)
-    if (parts < 2) return w;
+    if (parts < 1) parts = 1;
     w.parts = parts;
     w.each = (vecs + parts - 1) / parts;
     w.record_bytes = 16 + (k * 8 + 15) / 16 * 16;
@@ -1526,7 +1528,7 @@ extern "C" int sfb_token_logprobs(sfb_stream_t stream, float* logprob, float* en
     hipStream_t s = (hipStream_t)stream;
     clear_stale_error();
     const uint32_t vecs = vocab / (dtype == SFB_BF16 ? 8u : 4u);
-    const SplitWork w = split_rows(workspace, rows, vecs, top_k);
+    const SplitWork w = split_rows(workspace, rows, vecs, top_k, 256);
     const bool is_short = vecs <= kShortVecs && top_k <= kShortTop;
     if (too_many(rows, is_short ? 256 / kShortRows : vecs <= 256 ? 64 : vecs <= 1024 ? 256 : 512)) return SFB_ERR_SHAPE;
     const dim3 grid((uint32_t)rows);
@@ -1608,8 +1610,8 @@ extern "C" int sfb_distillation_loss(sfb_stream_t stream, float* row_loss, float
     hipStream_t s = (hipStream_t)stream;
     clear_stale_error();
     const uint32_t vecs = vocab / (dtype == SFB_BF16 ? 8u : 4u);
-    const SplitWork w = split_rows(d_logits && vecs <= kSplitGradient ? nullptr : workspace, rows, vecs, 0);
-    if (w.parts > 1) {   // the loss, then the gradient from the rows' statistics
+    const SplitWork w = split_rows(workspace, rows, vecs, 0, 512);
+    if (d_logits ? w.parts > 0 && vecs > kSplitGradient : w.parts > 1) {   // the loss, then the gradient from the rows' statistics
         if (!stats) p.stats = w.stats;
         const dim3 parts((uint32_t)rows * w.parts);
         if (dtype == SFB_F32) distill_split_kernel<float><<<parts, kSplitThreads, 0, s>>>(p, w);
@@ -1634,6 +1636,7 @@ extern "C" int sfb_distillation_loss(sfb_stream_t stream, float* row_loss, float
         else if (shape.threads == 256) distill_kernel<T, 256, 8, true><<<grid, 256, 0, s>>>(p);                    \
         else if (shape.threads == 512) distill_kernel<T, 512, 8, true><<<grid, 512, 0, s>>>(p);                    \
         else if (shape.vecs == 8) distill_kernel<T, 1024, 8, true><<<grid, 1024, 0, s>>>(p);                       \
+        else if (shape.vecs == 12) distill_kernel<T, 1024, 12, true><<<grid, 1024, 0, s>>>(p);                     \
         else if (shape.vecs == 16) distill_kernel<T, 1024, 16, true><<<grid, 1024, 0, s>>>(p);                     \
         else distill_kernel<T, 1024, 0, true><<<grid, 1024, 0, s>>>(p);                                            \
     } while (0)
