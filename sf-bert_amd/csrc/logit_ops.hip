@@ -1227,7 +1227,6 @@ struct GradParams {
 };
 
 constexpr int kGradThreads = 256, kGradVecs = 4;
-constexpr uint32_t kSplitGradient = 8192;   // vectors up to which a row's loss and gradient stay one launch
 
 // One work-group per kGradThreads * kGradVecs vectors of a row.
 template <typename T, bool ENTROPY, bool TEACHER>
@@ -1502,6 +1501,12 @@ static inline int check_logits(const void* logits, int dtype, uint64_t rows, uin
     if (workspace && workspace_bytes < SFB_LOGIT_WORKSPACE_BYTES) return SFB_ERR_WORKSPACE;
     return SFB_OK;
 }
+// Whether a gradient's rows are launched twice, cut for the loss and then for the gradient, instead of each by one
+// work-group that keeps it.  bf16 rows: 20 of 8125 vectors 12.6 us cut and 11.7 whole, 20 of 12500 13.6 and 16.3, 100 of
+// 12500 18.5 and 18.0, 500 of 12500 58 and 45; rows past 16384 vectors, which no work-group holds (fp32): 300 of 32768 85
+// and 102, 4 of them 11 and 21.
+static inline bool loss_first(uint64_t rows, uint32_t vecs) { return vecs > 16384 || (vecs > 8192 && rows <= 64); }
+
 // A launch has fewer than 2^32 threads.
 static inline bool too_many(uint64_t groups, uint32_t threads) { return groups * threads > 0xffffffffull; }
 static inline bool misaligned4(const void* a, const void* b = nullptr, const void* c = nullptr, const void* d = nullptr) {
@@ -1611,7 +1616,7 @@ extern "C" int sfb_distillation_loss(sfb_stream_t stream, float* row_loss, float
     clear_stale_error();
     const uint32_t vecs = vocab / (dtype == SFB_BF16 ? 8u : 4u);
     const SplitWork w = split_rows(workspace, rows, vecs, 0, 512);
-    if (d_logits ? w.parts > 0 && vecs > kSplitGradient : w.parts > 1) {   // the loss, then the gradient from the rows' statistics
+    if (d_logits ? w.parts > 0 && loss_first(rows, vecs) : w.parts > 1) {
         if (!stats) p.stats = w.stats;
         const dim3 parts((uint32_t)rows * w.parts);
         if (dtype == SFB_F32) distill_split_kernel<float><<<parts, kSplitThreads, 0, s>>>(p, w);
