@@ -719,7 +719,7 @@ template <typename T, int THREADS> struct NamedLogits {
         for (int r = 0; r < ROUNDS; ++r) {
             const uint32_t i = threadIdx.x + r * THREADS;
             id[r] = -1;
-            if (i < n) id[r] = ids[i];
+            if (r * THREADS < (int)n && i < n) id[r] = ids[i];
         }
     }
     __device__ __forceinline__ void load_logits(const RowSpan<T>& span, uint32_t vocab) {
@@ -1078,17 +1078,36 @@ struct RowGrad {
 };
 
 // The tokens that a row's coefficients belong to, and those coefficients, in shared memory, filled up with id -1 to a
-// whole number of fours.
+// whole number of fours.  Tokens named more than once are rare but have to add up: a bit per token (its lower 13 bits)
+// tells the slots that come second to one, and only tokens that such a slot names are searched for in the whole list.
+// (Every slot searching cost ten times the row itself at 3339 logits and 150 slots.)
 struct Slots {
     int32_t id[kMaxSlots];
     float coef[kMaxSlots];
-};
-template <int THREADS> __device__ __forceinline__ void pad_slots(Slots& slots, uint32_t n) {
-    if (n + threadIdx.x < (n + 3) / 4 * 4) {   // (at most three)
-        slots.id[n + threadIdx.x] = -1;
-        slots.coef[n + threadIdx.x] = 0.f;
+    uint32_t seen[256];
+    int32_t again[kMaxSlots];
+    uint32_t n_again;
+
+    // three steps with a barrier after each: put() every slot, mark() every slot, then the rest of it can be read
+    __device__ __forceinline__ void put(uint32_t i, int32_t token) {
+        id[i] = token;
+        seen[(uint32_t)token >> 5 & 255u] = 0;
     }
-}
+    template <int THREADS> __device__ __forceinline__ void finish(uint32_t n) {
+        const uint32_t t = threadIdx.x;
+        if (n + t < (n + 3) / 4 * 4) {   // (at most three)
+            id[n + t] = -1;
+            coef[n + t] = 0.f;
+        }
+        if (t == 0) n_again = 0;
+    }
+    __device__ __forceinline__ void mark(int32_t token, uint32_t vocab) {
+        if ((uint32_t)token >= vocab) return;
+        const uint32_t bit = 1u << ((uint32_t)token & 31u);
+        const uint32_t before = __hip_atomic_fetch_or(&seen[(uint32_t)token >> 5 & 255u], bit, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        if (before & bit) again[__hip_atomic_fetch_add(&n_again, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP)] = token;
+    }
+};
 // The gradient's entries that tokens name: equal tokens add up in slot order, and the first of them writes the entry.
 template <typename T, int THREADS> struct NamedEntries {
     static constexpr uint32_t ROUNDS = THREADS < (int)kMaxSlots ? kMaxSlots / THREADS : 1;
@@ -1096,23 +1115,28 @@ template <typename T, int THREADS> struct NamedEntries {
     int32_t id[ROUNDS];   // -1: nothing to write
     // sums of the coefficients of this thread's tokens in elements [e0, e1)
     __device__ __forceinline__ void total(const Slots& slots, uint32_t n, uint32_t e0, uint32_t e1) {
+        const uint32_t many = slots.n_again;
 #pragma unroll
         for (uint32_t r = 0; r < ROUNDS; ++r) {
             const uint32_t i = threadIdx.x + r * THREADS;
             id[r] = -1;
             value[r] = 0.f;
-            if (i >= n) continue;
+            if (r * THREADS >= n || i >= n) continue;
             const int32_t mine = slots.id[i];
             if (mine < 0 || (uint32_t)mine < e0 || (uint32_t)mine >= e1) continue;
-            float sum = 0.f;
-            bool first = true;
+            bool alone = true, first = true;
+            for (uint32_t k = 0; k < many; ++k) alone = alone && slots.again[k] != mine;
+            float sum = slots.coef[i];
+            if (!alone) {
+                sum = 0.f;
 #pragma unroll 2
-            for (uint32_t k = 0; k < n; k += 4) {
+                for (uint32_t k = 0; k < n; k += 4) {
 #pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) {
-                    const bool same = slots.id[k + j] == mine;
-                    sum += same ? slots.coef[k + j] : 0.f;
-                    first = first && !(same && k + j < i);
+                    for (uint32_t j = 0; j < 4; ++j) {
+                        const bool same = slots.id[k + j] == mine;
+                        sum += same ? slots.coef[k + j] : 0.f;
+                        first = first && !(same && k + j < i);
+                    }
                 }
             }
             if (first) id[r] = mine;
@@ -1178,7 +1202,7 @@ struct Teacher {
         for (uint32_t r = 0; r < ROUNDS; ++r) {
             const uint32_t i = lane + 64 * r;
             v[r] = -kInf;
-            if (i < n) {
+            if (64 * r < n && i < n) {
                 const int32_t id = ids[i];
                 if (id >= 0 && (uint32_t)id < vocab) v[r] = as_bf16 ? bf16_bits_to_f32(bits[r]) : __builtin_bit_cast(float, bits[r]);
             }
@@ -1188,14 +1212,14 @@ struct Teacher {
         float sum = 0.f;
 #pragma unroll
         for (uint32_t r = 0; r < ROUNDS; ++r)
-            if (v[r] != -kInf) sum += exp2_fast((v[r] - hi) * c);
+            if (64 * r < n && v[r] != -kInf) sum += exp2_fast((v[r] - hi) * c);
         sum = wave_sum(sum);
         const float l = log2f(sum);
         minus_entropy = 0.f;
 #pragma unroll
         for (uint32_t r = 0; r < ROUNDS; ++r) {
             const uint32_t i = lane + 64 * r;
-            if (i < n) {
+            if (64 * r < n && i < n) {
                 float qi = 0.f;
                 if (v[r] != -kInf) {
                     const float lq = (v[r] - hi) * c - l;
@@ -1226,12 +1250,12 @@ struct GradParams {
     float scale, c;
 };
 
-constexpr int kGradThreads = 256, kGradVecs = 4;
+constexpr int kGradVecs = 4;
 
-// One work-group per kGradThreads * kGradVecs vectors of a row.
-template <typename T, bool ENTROPY, bool TEACHER>
-__global__ __launch_bounds__(kGradThreads) void logit_gradient_kernel(GradParams p) {
-    constexpr int THREADS = kGradThreads, NV = kGradVecs;
+// One work-group per THREADS * kGradVecs vectors of a row.
+template <typename T, int THREADS, bool ENTROPY, bool TEACHER>
+__global__ __launch_bounds__(THREADS) void logit_gradient_kernel(GradParams p) {
+    constexpr int NV = kGradVecs;
     __shared__ float red[2 * THREADS / 64];
     __shared__ Slots slots;
     __shared__ uint32_t some_teacher;
@@ -1253,14 +1277,15 @@ __global__ __launch_bounds__(kGradThreads) void logit_gradient_kernel(GradParams
     if (TEACHER) {
         Teacher teacher;
         if (t < 64) teacher.load(p.teacher, p.teacher_bf16, row * p.n, p.n);
-        for (uint32_t i = t; i < p.n; i += THREADS) slots.id[i] = p.ids[row * p.n + i];
+        for (uint32_t i = t; i < p.n; i += THREADS) slots.put(i, p.ids[row * p.n + i]);
+        slots.template finish<THREADS>(p.n);
         held.load(span, s, t);
         __syncthreads();
+        for (uint32_t i = t; i < p.n; i += THREADS) slots.mark(slots.id[i], p.vocab);
         if (t < 64) {
             teacher.softmax(slots.id, p.teacher_bf16, p.n, p.vocab, p.c, slots.coef);
             if (t == 0) some_teacher = teacher.some ? 1u : 0u;
         }
-        pad_slots<THREADS>(slots, p.n);
         __syncthreads();
         if (!some_teacher) {
             write_zeros<T, THREADS>(span, s, d);
@@ -1276,12 +1301,16 @@ __global__ __launch_bounds__(kGradThreads) void logit_gradient_kernel(GradParams
             const int32_t id = p.ids[row * p.n + i];
             const float v = p.d_logprob[row * p.n + i];
             const bool inside = id >= 0 && (uint32_t)id < p.vocab;
-            slots.id[i] = id;
+            slots.put(i, id);
             slots.coef[i] = inside ? v : 0.f;
             if (inside) { C += v; any += v != 0.f ? 1.f : 0.f; }
         }
-        pad_slots<THREADS>(slots, p.n);
-        group_sum<THREADS, true>(C, any, red);   // (its barriers complete the slots too)
+        slots.template finish<THREADS>(p.n);
+        __syncthreads();
+        if (p.n > 1)
+            for (uint32_t i = t; i < p.n; i += THREADS) slots.mark(slots.id[i], p.vocab);
+        group_sum<THREADS, true>(C, any, red);
+        __syncthreads();
         if (any == 0.f && ent == 0.f) {
             write_zeros<T, THREADS>(span, s, d);
             return;
@@ -1340,10 +1369,11 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 && NV == 8 ? 8 : 4) void d
 #pragma unroll
     for (int r = 0; r < logits.ROUNDS; ++r) {
         const uint32_t i = t + r * THREADS;
-        if (i < p.n) slots.id[i] = logits.id[r];
+        if (i < p.n) slots.put(i, logits.id[r]);
         if ((uint32_t)logits.id[r] < p.vocab) used = 1.f;
     }
-    used = group_max<THREADS>(used, red, [&]() { pad_slots<THREADS>(slots, p.n); });
+    slots.template finish<THREADS>(p.n);
+    used = group_max<THREADS>(used, red, []() {});
     if (used == 0.f) {   // no slot (padding): the logits are not read
         if (t == 0) {
             p.row_loss[row] = 0.f;
@@ -1351,6 +1381,10 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 && NV == 8 ? 8 : 4) void d
         }
         if (GRAD) write_zeros<T, THREADS>(span, s, d);
         return;
+    }
+    if (GRAD) {
+#pragma unroll
+        for (int r = 0; r < logits.ROUNDS; ++r) slots.mark(logits.id[r], p.vocab);
     }
     logits.load_logits(span, p.vocab);
     NamedEntries<T, THREADS> named;
@@ -1423,7 +1457,7 @@ template <typename T> __global__ __launch_bounds__(kSplitThreads, 8) void distil
     if (t < 64) teacher.load(p.teacher, p.teacher_bf16, row * p.n, p.n);
     logits.load_ids(p.ids + row * p.n, p.n);
     float used = 0.f;
-    if (t < p.n) slots.id[t] = logits.id[0];
+    if (t < p.n) slots.put(t, logits.id[0]);
     if ((uint32_t)logits.id[0] < p.vocab) used = 1.f;
     used = group_max<THREADS>(used, red, []() {});
     if (used == 0.f) {
@@ -1460,7 +1494,8 @@ static inline RowShape distill_shape(uint32_t vocab, int dtype, bool gradient) {
     const uint32_t vecs = vocab / (dtype == SFB_BF16 ? 8u : 4u);
     if (vecs <= 64) return {64, 1};
     if (vecs <= 256) return {64, 4};
-    if (vecs <= 1024) return {256, 4};
+    if (vecs <= 512) return {64, 8};
+    if (vecs <= 1024) return {128, 8};
     if (!gradient) return {512, 0};
     if (vecs <= 2048) return {256, 8};
     if (vecs <= 4096) return {512, 8};
@@ -1535,7 +1570,7 @@ extern "C" int sfb_token_logprobs(sfb_stream_t stream, float* logprob, float* en
     const uint32_t vecs = vocab / (dtype == SFB_BF16 ? 8u : 4u);
     const SplitWork w = split_rows(workspace, rows, vecs, top_k, 256);
     const bool is_short = vecs <= kShortVecs && top_k <= kShortTop;
-    if (too_many(rows, is_short ? 256 / kShortRows : vecs <= 256 ? 64 : vecs <= 1024 ? 256 : 512)) return SFB_ERR_SHAPE;
+    if (too_many(rows, is_short ? 256 / kShortRows : vecs <= 512 ? 64 : vecs <= 1024 ? 128 : 512)) return SFB_ERR_SHAPE;
     const dim3 grid((uint32_t)rows);
 #define SFB_LP_AS(T, ENT)                                                                                              \
     do {                                                                                                               \
@@ -1545,7 +1580,8 @@ extern "C" int sfb_token_logprobs(sfb_stream_t stream, float* logprob, float* en
             token_logprobs_short_kernel<T, ENT><<<dim3((uint32_t)((rows + kShortRows - 1) / kShortRows)), 256, 0, s>>>(p, (uint32_t)rows); \
         else if (vecs <= 64) token_logprobs_held_kernel<T, 64, 1, ENT><<<grid, 64, 0, s>>>(p);                         \
         else if (vecs <= 256) token_logprobs_held_kernel<T, 64, 4, ENT><<<grid, 64, 0, s>>>(p);                        \
-        else if (vecs <= 1024) token_logprobs_held_kernel<T, 256, 4, ENT><<<grid, 256, 0, s>>>(p);                     \
+        else if (vecs <= 512) token_logprobs_held_kernel<T, 64, 8, ENT><<<grid, 64, 0, s>>>(p);                        \
+        else if (vecs <= 1024) token_logprobs_held_kernel<T, 128, 8, ENT><<<grid, 128, 0, s>>>(p);                     \
         else if (top_k && vecs <= 4096) token_logprobs_stream_kernel<T, 256, ENT><<<grid, 256, 0, s>>>(p);             \
         else token_logprobs_stream_kernel<T, 512, ENT><<<grid, 512, 0, s>>>(p);                                        \
     } while (0)
@@ -1563,20 +1599,27 @@ extern "C" int sfb_token_logprobs(sfb_stream_t stream, float* logprob, float* en
 
 static int launch_gradient(hipStream_t s, GradParams& p, int dtype, uint64_t rows, bool entropy, bool teacher) {
     const uint32_t vecs = p.vocab / (dtype == SFB_BF16 ? 8u : 4u);
-    p.each = kGradThreads * kGradVecs;
+    const uint32_t threads = vecs <= 256 ? 64 : 256;
+    p.each = threads * kGradVecs;
     p.parts = vecs == 0 ? 1 : (vecs + p.each - 1) / p.each;
-    if (too_many(rows * p.parts, kGradThreads)) return SFB_ERR_SHAPE;
+    if (too_many(rows * p.parts, threads)) return SFB_ERR_SHAPE;
     const dim3 grid((uint32_t)(rows * p.parts));
     clear_stale_error();
-#define SFB_GR(T)                                                                                       \
-    do {                                                                                                \
-        if (teacher) logit_gradient_kernel<T, false, true><<<grid, kGradThreads, 0, s>>>(p);             \
-        else if (entropy) logit_gradient_kernel<T, true, false><<<grid, kGradThreads, 0, s>>>(p);        \
-        else logit_gradient_kernel<T, false, false><<<grid, kGradThreads, 0, s>>>(p);                    \
+#define SFB_GR_AS(T, TH)                                                                               \
+    do {                                                                                               \
+        if (teacher) logit_gradient_kernel<T, TH, false, true><<<grid, TH, 0, s>>>(p);                 \
+        else if (entropy) logit_gradient_kernel<T, TH, true, false><<<grid, TH, 0, s>>>(p);            \
+        else logit_gradient_kernel<T, TH, false, false><<<grid, TH, 0, s>>>(p);                        \
+    } while (0)
+#define SFB_GR(T)                              \
+    do {                                       \
+        if (threads == 64) SFB_GR_AS(T, 64);   \
+        else SFB_GR_AS(T, 256);                \
     } while (0)
     if (dtype == SFB_F32) SFB_GR(float);
     else SFB_GR(__bf16);
 #undef SFB_GR
+#undef SFB_GR_AS
     return launch_status();
 }
 
@@ -1635,8 +1678,9 @@ extern "C" int sfb_distillation_loss(sfb_stream_t stream, float* row_loss, float
 #define SFB_DL_AS(T, GRAD)                                                                                         \
     do {                                                                                                           \
         if (shape.threads == 64 && shape.vecs == 1) distill_kernel<T, 64, 1, GRAD><<<grid, 64, 0, s>>>(p);         \
-        else if (shape.threads == 64) distill_kernel<T, 64, 4, GRAD><<<grid, 64, 0, s>>>(p);                       \
-        else if (shape.threads == 256 && shape.vecs == 4) distill_kernel<T, 256, 4, GRAD><<<grid, 256, 0, s>>>(p); \
+        else if (shape.threads == 64 && shape.vecs == 4) distill_kernel<T, 64, 4, GRAD><<<grid, 64, 0, s>>>(p);    \
+        else if (shape.threads == 64) distill_kernel<T, 64, 8, GRAD><<<grid, 64, 0, s>>>(p);                       \
+        else if (shape.threads == 128) distill_kernel<T, 128, 8, GRAD><<<grid, 128, 0, s>>>(p);                    \
         else if (!GRAD) distill_kernel<T, 512, 0, false><<<grid, 512, 0, s>>>(p);                                  \
         else if (shape.threads == 256) distill_kernel<T, 256, 8, true><<<grid, 256, 0, s>>>(p);                    \
         else if (shape.threads == 512) distill_kernel<T, 512, 8, true><<<grid, 512, 0, s>>>(p);                    \

@@ -247,3 +247,4 @@ inline void emu_atomic_store(T* p, V v) {
 #define __hip_atomic_load(p, order, scope) emu_atomic_load(p)
 #define __hip_atomic_store(p, v, order, scope) emu_atomic_store(p, v)
 #define __hip_atomic_fetch_add(p, v, order, scope) __atomic_fetch_add(p, v, order)
+#define __hip_atomic_fetch_or(p, v, order, scope) __atomic_fetch_or(p, v, order)
