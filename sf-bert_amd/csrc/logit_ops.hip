@@ -702,9 +702,11 @@ struct LogprobParams {
     float scale, c;
 };
 
+// Half the distance of a logit from the reference: the distance itself may pass the largest fp32.
+__device__ __forceinline__ float half_distance(float x, float m) { return 0.5f * x - 0.5f * m; }
 // ln p of a logit x from a row's statistics; a row without any logit above -inf gives -inf
 __device__ __forceinline__ float log_prob(float x, float m, float l, float scale) {
-    return l == -kInf ? -kInf : (x - m) * scale - l * kLn2;
+    return l == -kInf ? -kInf : half_distance(x, m) * (2.f * scale) - l * kLn2;
 }
 
 // The logits of a row's tokens, one per thread, fetched before the row is read: by the time its sums are known they
@@ -924,18 +926,17 @@ __global__ __launch_bounds__(256) void token_logprobs_short_kernel(LogprobParams
 #pragma unroll
         for (int e = 0; e < E; ++e) mine = mine > order[e] ? mine : order[e];
         const uint32_t best = over16(mine, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
-        uint32_t index = 0xffffffffu;   // the lowest one that has it
+        // the lowest element that has it: this lane's (an edge element may be the row's first ones or its last), then all
+        uint32_t at = E, index = 0xffffffffu;
 #pragma unroll
-        for (int e = E - 1; e >= 0; --e) {
-            const uint32_t j = e == E - 1 ? (uint32_t)edge : span.index(g + 16 * (e / N)) + e % N;
-            if (order[e] == best && j < index) index = j;
-        }
+        for (int e = E - 2; e >= 0; --e) at = order[e] == best ? e : at;
+        if (at != E) index = span.index(g + 16 * (at / N)) + at % N;
+        if (order[E - 1] == best && (uint32_t)edge < index) { at = E - 1; index = (uint32_t)edge; }
+        const uint32_t own = index;
         index = over16(index, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+        if (own != index) at = E;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const uint32_t j = e == E - 1 ? (uint32_t)edge : span.index(g + 16 * (e / N)) + e % N;
-            if (j == index) order[e] = 0;
-        }
+        for (int e = 0; e < E; ++e) order[e] = at == e ? 0 : order[e];
         if (g == 0 && writes) {
             p.top_ids[row * p.top_k + k] = (int32_t)index;
             p.top_logprobs[row * p.top_k + k] = log_prob(logit_of(best), r.m, l, p.scale);
@@ -1341,16 +1342,15 @@ struct DistillParams {
     float scale, c;
 };
 
-// cross: sum q (x - m) s.  (No logit above -inf: the student gives the teacher's tokens no probability.)
+// cross: sum q (x - m) / 2.  (No logit above -inf: the student gives the teacher's tokens no probability.)
 __device__ __forceinline__ float row_loss(const Teacher& teacher, float l, float cross, float scale) {
-    const float loss = l == -kInf ? kInf : (teacher.minus_entropy + l) * kLn2 - cross;
-    return loss / (scale * scale);
+    return l == -kInf ? kInf : (teacher.minus_entropy + l) * kLn2 / (scale * scale) - cross * (2.f / scale);
 }
 
 // One work-group per row, held in registers (NV vectors per thread) or, NV = 0, streamed: the student's sums, the loss,
 // and (GRAD) the gradient, for which a held row is not read again.  The teacher's softmax and the logits of its tokens
 // are ready by the time the row has arrived; with m, l of the student and q of the teacher the loss is
-//   ( sum q ln q - sum q (x - m) s + ln2 l ) / s^2.
+//   ( sum q ln q + ln2 l ) / s^2 - sum q (x - m) / s.
 template <typename T, int THREADS, int NV, bool GRAD>
 __global__ __launch_bounds__(THREADS, THREADS == 1024 && NV == 8 ? 8 : 4) void distill_kernel(DistillParams p) {
     __shared__ float red[2 * THREADS / 64];
@@ -1395,7 +1395,7 @@ __global__ __launch_bounds__(THREADS, THREADS == 1024 && NV == 8 ? 8 : 4) void d
         for (int r = 0; r < logits.ROUNDS; ++r) {
             const uint32_t i = t + r * THREADS;
             const float q = i < p.n ? slots.coef[i] : 0.f;
-            if (!(q <= 0.f)) cross += q * ((LogitVec<T>::value(logits.x[r]) - m) * p.scale);
+            if (!(q <= 0.f)) cross += q * half_distance(LogitVec<T>::value(logits.x[r]), m);
         }
         if (GRAD) named.total(slots, p.n, 0, p.vocab);
         return cross;
@@ -1479,7 +1479,7 @@ template <typename T> __global__ __launch_bounds__(kSplitThreads, 8) void distil
     const float m = joined[0], l = log2f(joined[1]);
     const float q = t < p.n ? slots.coef[t] : 0.f;
     float cross = 0.f, unused = 0.f;
-    if (!(q <= 0.f)) cross = q * ((LogitVec<T>::value(logits.x[0]) - (m == -kInf ? 0.f : m)) * p.scale);
+    if (!(q <= 0.f)) cross = q * half_distance(LogitVec<T>::value(logits.x[0]), m == -kInf ? 0.f : m);
     group_sum<THREADS, false>(cross, unused, red);
     if (t == 0) {
         p.row_loss[row] = teacher.some ? row_loss(teacher, l, cross, p.scale) : 0.f;

@@ -179,8 +179,15 @@ def logprob_tol(x, scale, want):
 # ---------------------------------------------------------------------------------------------------------------
 # cases
 # ---------------------------------------------------------------------------------------------------------------
-def tokens_of(rng, rows, vocab, n):
+def alike(ids, vocab):
+    """Few different tokens, most of them several times, and with equal lower 13 bits where the vocabulary has such."""
+    return (ids % 3 % vocab + 8192 * (ids // 3 % max((vocab - 3) // 8192 + 1, 1))).astype(np.int32)
+
+
+def tokens_of(rng, rows, vocab, n, few=False):
     ids = rng.integers(0, vocab, (rows, n)).astype(np.int32)
+    if few:
+        ids = alike(ids, vocab)
     if n > 2:
         ids[:, 1] = ids[:, 0]          # the same token twice
         ids[::2, 2] = -100             # no token
@@ -188,11 +195,12 @@ def tokens_of(rng, rows, vocab, n):
     return ids
 
 
-def logprobs(S, dev, vocab, bf16, pad=0, n=1, k=4, scale=1.0, workspace=None, kinds=KINDS, seed=1, repeat=1, entropy=True):
+def logprobs(S, dev, vocab, bf16, pad=0, n=1, k=4, scale=1.0, workspace=None, kinds=KINDS, seed=1, repeat=1, entropy=True,
+             few=False):
     rng = np.random.default_rng(seed)
     x = matrix(vocab, seed + 1, bf16, kinds)
     rows = x.shape[0]
-    ids = tokens_of(rng, rows, vocab, n)
+    ids = tokens_of(rng, rows, vocab, n, few)
     t = on_device(dev, x, bf16, pad)
     lp = plain_log_softmax(x, scale)
     tok = dev(ids[:, 0].copy() if n == 1 else ids)
@@ -231,8 +239,8 @@ def gradient_tol(x, scale, lp, weight, want, bf16):
     return tol + (2.0 ** -8 * np.abs(np.nan_to_num(want)) + 2.0 ** -127 if bf16 else 2.0 ** -126)
 
 
-def logprobs_backward(S, dev, vocab, bf16, pad=0, n=1, scale=1.0, entropy=True, in_place=False, kinds=KINDS, seed=5):
-    t, tok, x, ids, lp, got = logprobs(S, dev, vocab, bf16, pad, n, 0, scale, kinds=kinds, seed=seed, entropy=entropy)
+def logprobs_backward(S, dev, vocab, bf16, pad=0, n=1, scale=1.0, entropy=True, in_place=False, kinds=KINDS, seed=5, few=False):
+    t, tok, x, ids, lp, got = logprobs(S, dev, vocab, bf16, pad, n, 0, scale, kinds=kinds, seed=seed, entropy=entropy, few=few)
     rng = np.random.default_rng(seed + 100)
     rows = x.shape[0]
     g = rng.standard_normal((rows, n)).astype(np.float32)
@@ -252,8 +260,10 @@ def logprobs_backward(S, dev, vocab, bf16, pad=0, n=1, scale=1.0, entropy=True, 
     return d
 
 
-def teacher_of(rng, rows, vocab, slots, teacher_bf16):
+def teacher_of(rng, rows, vocab, slots, teacher_bf16, few=False):
     ids = rng.integers(0, vocab, (rows, slots)).astype(np.int32)
+    if few:
+        ids = alike(ids, vocab)
     z = (rng.standard_normal((rows, slots)) * 2 + 3).astype(np.float32)
     if slots > 3:
         ids[:, 1] = ids[:, 0]           # the same token twice
@@ -267,11 +277,11 @@ def teacher_of(rng, rows, vocab, slots, teacher_bf16):
 
 
 def distillation(S, dev, vocab, bf16, pad=0, slots=8, scale=0.5, teacher_bf16=False, in_place=False, workspace=None,
-                 kinds=KINDS, seed=9, repeat=1):
+                 kinds=KINDS, seed=9, repeat=1, few=False):
     rng = np.random.default_rng(seed)
     x = matrix(vocab, seed + 1, bf16, kinds)
     rows = x.shape[0]
-    ids, z = teacher_of(rng, rows, vocab, slots, teacher_bf16)
+    ids, z = teacher_of(rng, rows, vocab, slots, teacher_bf16, few)
     w = rng.standard_normal(rows).astype(np.float32)
     w[-1] = 0.0
     loss, lp, q = plain_distill(x, ids, z, scale)
@@ -354,6 +364,39 @@ def parts_left_out(S, dev):
     with np.errstate(all="ignore"):
         weight = np.abs(ge) * (20 + 2 * np.nan_to_num(plain_entropy(lp)))
     same(host(d), want, gradient_tol(x, 1.0, lp, weight, want, False), "entropy's gradient")
+
+
+def far_apart(S, dev, vocab, bf16, workspace=None):
+    """Logits whose distance is past the largest fp32, though its product with a small scale, or its quotient by a large
+    one, is not."""
+    rng = np.random.default_rng(61)
+    low, x = LOWEST[bf16], np.zeros((3, vocab), np.float32)
+    x[:2, vocab // 3] = -low
+    x[:, vocab // 2] = low
+    x[1, 2::5] = low
+    x[2] = low
+    x[2, vocab - 1] = -low
+    t = dev(x, bf16)
+    ids = np.tile(np.int32([vocab // 3, vocab // 2, 0, vocab - 1]), (3, 1))
+    for scale in (1e-4, 1e-3):
+        lp = plain_log_softmax(x, scale)
+        got = S.token_logprobs(t, dev(ids), top_k=3, scale=scale, entropy=True, workspace=workspace)
+        want = np.take_along_axis(lp, ids.astype(np.int64), 1)
+        assert np.isfinite(want).all() and want.min() < -1e34
+        same(host(got["logprob"]), want, logprob_tol(x, scale, want), "logprob")
+        assert (host(got["entropy"]) == 0).all()   # one token has all of the probability
+        assert np.array_equal(host(got["top_ids"]), plain_top(x, 3))
+        want = np.take_along_axis(lp, plain_top(x, 3), 1)
+        same(host(got["top_logprobs"]), want, logprob_tol(x, scale, want), "top_logprobs")
+    z = rng.standard_normal((3, 4)).astype(np.float32)
+    for scale in (2.5, 40.0):   # loss: sum q (distance) / scale, 8 roundings of it beside the slots' 4
+        loss, lp, q = plain_distill(x, ids, z, scale)
+        assert np.isfinite(loss.astype(np.float32)).all() and loss.max() > 1e30
+        w = dev(np.ones(3, np.float32))
+        for d_loss in (None, w):
+            got = S.distillation_loss(t, dev(ids), dev(z), scale=scale, d_loss=d_loss, workspace=workspace)
+            # (q's error: 5 u |t| + (slots + 40) u relative, |t| the teacher's largest exponent)
+            same(host(got["row_loss"]), loss, U * (12 + 44 + 5 * 8 * scale) * np.abs(loss), "row_loss")
 
 
 def refusals(S, dev):

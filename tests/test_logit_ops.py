@@ -10,7 +10,8 @@ from test_emulated_kernels import E   # noqa: F401  (fixture: the host build)
 
 # vocabulary, bf16, padding of the rows: a wave, four waves and sixteen waves per row, sizes around a vector, odd ones
 SHAPES = [(1, False, 0), (1, True, 3), (5, True, 0), (7, False, 2), (16, True, 0), (50, False, 0), (257, True, 0),
-          (1000, False, 24), (2047, False, 0), (2051, False, 0), (4099, True, 0), (4096, True, 8), (9001, False, 1),
+          (1000, False, 24), (2047, False, 0), (2051, False, 0), (2999, False, 5), (4099, True, 0), (4096, True, 8),
+          (7003, True, 1), (9001, False, 1),
           (30522, True, 0), (30522, False, 6), (70001, False, 0), (140001, True, 0)]
 ON_HOST = [s for s in SHAPES if s[0] < 10000]
 
@@ -73,6 +74,26 @@ def test_few_long_rows_cut_over_the_device(vocab, bf16, pad):
         cases.distillation(S, dev, vocab, bf16, pad, slots=slots, teacher_bf16=teacher_bf16, in_place=in_place, workspace=ws, seed=30 + slots)
     torch.cuda.synchronize()
     assert int(ws[:2048].view(torch.int32).abs().sum()) == 0, "arrival counters must be left at zero"
+
+
+# the same token several times, and tokens that the search for those cannot tell apart at first
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab,bf16", [(3, False), (700, True), (2999, False), (30522, True), (70001, False), (140001, True)])
+def test_few_tokens_named_many_times_on_the_device(vocab, bf16):
+    for n in (2, 67, 256):
+        cases.logprobs_backward(*device_backend(), vocab, bf16, 0, n=n, few=True, seed=70 + n)
+        cases.distillation(*device_backend(), vocab, bf16, 1, slots=n, few=True, seed=71 + n)
+
+
+FAR_APART = [(11, False), (200, True), (1000, False), (2500, False), (9001, True), (40000, False)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab,bf16", FAR_APART)
+def test_logits_far_apart_on_the_device(vocab, bf16):
+    S, dev = device_backend()
+    cases.far_apart(S, dev, vocab, bf16)
+    cases.far_apart(S, dev, vocab, bf16, workspace=torch.zeros(S.LOGIT_WORKSPACE_BYTES, dtype=torch.uint8, device="cuda"))
 
 
 @pytest.mark.gpu
@@ -258,6 +279,22 @@ def test_logit_ops_with_lanes_in_adverse_orders(E, order):   # noqa: F811
     cases.logprobs_backward(*back, 2500, False, 1, n=5, in_place=True)
     cases.distillation(*back, 4200, True, 3, slots=70, in_place=True)
     cases.distillation(*back, 900, False, 0, slots=70, in_place=True)
+
+
+@pytest.mark.parametrize("vocab,bf16,order", [(3, False, 0), (700, True, 14), (2999, False, 1), (9001, True, 0)])
+def test_few_tokens_named_many_times_on_the_host_model(E, vocab, bf16, order):   # noqa: F811
+    back = host_backend(E, order=order)
+    some = ["normal", "masked", "nan", "lowest", "empty"]
+    for n in (2, 67):
+        cases.logprobs_backward(*back, vocab, bf16, 0, n=n, few=True, seed=70 + n, kinds=some)
+        cases.distillation(*back, vocab, bf16, 1, slots=n, few=True, seed=71 + n, kinds=some)
+
+
+@pytest.mark.parametrize("vocab,bf16", FAR_APART[:-1])
+def test_logits_far_apart_on_the_host_model(E, vocab, bf16):   # noqa: F811
+    S, dev = host_backend(E)
+    cases.far_apart(S, dev, vocab, bf16)
+    cases.far_apart(S, dev, vocab, bf16, workspace=dev(np.zeros(S.LOGIT_WORKSPACE_BYTES, np.uint8)))
 
 
 def test_teacher_to_student_on_the_host_model(E):   # noqa: F811
