@@ -438,6 +438,7 @@ template <typename T, int THREADS> struct Streamed {
 
 // Order of the alternatives as whole numbers: larger logits first, -0 as +0, NaN above everything; 0 is below every
 // logit.  A composite's low word is the complement of the index: of equal logits the lowest index comes first.
+constexpr uint32_t kMaskedOrder = 0x007fffffu;   // of -inf
 __device__ __forceinline__ uint32_t order_of(float x) {
     const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.f);
     if ((b & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
@@ -458,13 +459,18 @@ template <typename T, int THREADS, int HELD> struct TopSelect {
     // (shared memory bounds how many short rows a compute unit works on at a time)
     static constexpr int VECTORS = HELD && HELD * THREADS < 256 ? HELD * THREADS : 256;
     static constexpr int LIST = HELD && HELD * THREADS * N + 16 < 512 ? HELD * THREADS * N + 16 : 512;
-    static constexpr int GROUPS = THREADS < 256 ? THREADS : 256;
+    // (one or two waves that hold a row give several groups each thread: with 64 groups and 64 alternatives the
+    // threshold is the least of the threads' maxima, 8000 rows of 2000 took 880 us for 25)
+    static constexpr int PER = HELD >= 4 && THREADS < 256 ? 256 / THREADS : 1;
+    static constexpr int GROUPS = THREADS * PER < 256 ? THREADS * PER : 256;
+    static constexpr uint32_t THIN = 128;
     static constexpr int LOW_BIT = sizeof(T) == 2 ? 16 : 0;   // bf16 logits are told apart by the upper half
+    static_assert(GROUPS <= VECTORS, "the groups share memory with the vectors");
     struct Shared {
         u32x4 vectors[VECTORS];       // vectors that hold a logit above the threshold
         uint64_t list[LIST];          // composites
-        uint32_t at[VECTORS];         // index of each vector's first element
-        uint32_t words[GROUPS + 2];   // the groups' largest logits, and what came of them
+        uint32_t at[VECTORS];         // index of each vector's first element; before: the groups' largest logits
+        uint32_t limit, exact;        // the threshold, and whether it is one of those
         uint32_t count, n_vectors;
     };
     static __device__ __forceinline__ Shared& shared() {
@@ -487,7 +493,7 @@ template <typename T, int THREADS, int HELD> struct TopSelect {
     template <int W> static __device__ __forceinline__ uint32_t search(uint32_t k, uint32_t* all) {
         uint32_t own[W], limit = 0;
 #pragma unroll
-        for (int i = 0; i < W; ++i) own[i] = shared().words[i * 64 + (threadIdx.x & 63)];
+        for (int i = 0; i < W; ++i) own[i] = shared().at[i * 64 + (threadIdx.x & 63)];
         *all = 1;
         for (int bit = 31; bit >= LOW_BIT; --bit) {
             const uint32_t next = limit | (1u << bit);
@@ -504,32 +510,38 @@ template <typename T, int THREADS, int HELD> struct TopSelect {
     // A threshold that at least k logits of the threads' largest reach, in three parts with a barrier after the first and
     // the second: every thread publishes its largest logit (and count is cleared), one wave searches, all read the
     // result; *exact: it is one of those logits.  Up to k = 32 the threads form 64 groups (k = 20: 24 logits expected
-    // above the threshold), beyond that up to 256.
-    static __device__ __forceinline__ void publish(float top, bool any, uint32_t k) {
+    // above the threshold), beyond that up to 256; own(i): order of the i-th of this thread's PER groups.
+    template <typename F> static __device__ __forceinline__ void publish(float top, bool any, uint32_t k, F own) {
         const uint32_t t = threadIdx.x;
+        if (PER > 1 && k > 32) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) shared().at[i * THREADS + t] = own(i);
+            if (t == 0) shared().count = shared().n_vectors = 0;
+            return;
+        }
         uint32_t mine = any ? order_of(top) : 0u;
-        const bool wide = THREADS > 64 && k > 32;
+        const bool wide = THREADS > 64 && k > 32;   // (THREADS >= 256)
         if (THREADS >= 128) mine = pair_max<0xB1>(mine, THREADS >= 512 || !wide);
         if (THREADS >= 256) mine = pair_max<0x4E>(mine, THREADS >= 1024 || !wide);
         if (THREADS >= 512 && !wide) mine = pair_max<0x141>(mine, true);
         if (THREADS >= 1024 && !wide) mine = pair_max<0x140>(mine, true);
         const uint32_t per = wide ? THREADS / GROUPS : THREADS / 64;
-        if (t % per == 0) shared().words[t / per] = mine;
+        if (t % per == 0) shared().at[t / per] = mine;
         if (t == 0) shared().count = shared().n_vectors = 0;
     }
     static __device__ __forceinline__ void find(uint32_t k) {
         if (threadIdx.x >= 64) return;
         uint32_t all;
-        const uint32_t limit = THREADS > 64 && k > 32 ? search<GROUPS / 64>(k, &all) : search<1>(k, &all);
-        if (threadIdx.x == 0) { shared().words[GROUPS] = limit; shared().words[GROUPS + 1] = all; }
+        const uint32_t limit = GROUPS > 64 && k > 32 ? search<GROUPS / 64>(k, &all) : search<1>(k, &all);
+        if (threadIdx.x == 0) { shared().limit = limit; shared().exact = all; }
     }
     static __device__ __forceinline__ uint32_t found(bool* exact) {
-        *exact = shared().words[GROUPS + 1] != 0;
-        return shared().words[GROUPS];
+        *exact = shared().exact != 0;
+        return shared().limit;
     }
     static __device__ __forceinline__ uint32_t threshold(float top, bool any, uint32_t k, bool* exact) {
         __syncthreads();
-        publish(top, any, k);
+        publish(top, any, k, [](int) { return 0u; });
         __syncthreads();
         find(k);
         __syncthreads();
@@ -593,12 +605,12 @@ template <typename T, int THREADS, int HELD> struct TopSelect {
             const bool equal = j < s.e1 && order == limit;
             const uint64_t in_wave = __builtin_amdgcn_ballot_w64(equal);
             __syncthreads();
-            if (lane == 0) shared().words[t >> 6] = (uint32_t)__builtin_popcountll(in_wave);
+            if (lane == 0) shared().at[t >> 6] = (uint32_t)__builtin_popcountll(in_wave);
             __syncthreads();
             uint32_t at = have + (uint32_t)__builtin_popcountll(in_wave & ((1ull << lane) - 1));
             for (uint32_t w = 0; w < THREADS / 64; ++w) {
-                if (w < (t >> 6)) at += shared().words[w];
-                have += shared().words[w];
+                if (w < (t >> 6)) at += shared().at[w];
+                have += shared().at[w];
             }
             if (equal && at < want) shared().list[above + at] = composite(order, j);
             return have < want;
@@ -642,7 +654,7 @@ template <typename T, int THREADS, int HELD> struct TopSelect {
     static __device__ __forceinline__ float early(float top, bool any, uint32_t k) {
         bool exact;
         const uint32_t limit = threshold(top, any, k, &exact);
-        return limit <= 0x007fffffu ? __builtin_nanf("") : logit_of(limit);
+        return limit <= kMaskedOrder ? __builtin_nanf("") : logit_of(limit);
     }
 
     static __device__ __forceinline__ void edge(const RowSpan<T>& span, const Slice& s, float least) {
@@ -651,19 +663,70 @@ template <typename T, int THREADS, int HELD> struct TopSelect {
             if (x >= least) append(order_of(x), (uint32_t)s.edge);
         }
     }
+    // Few threads and many alternatives: the threshold lets most of a row through, and ranking n logits costs n^2.  One
+    // wave finds the k-th largest of the list and keeps those that reach it.
+    static __device__ __forceinline__ void thin_out(uint32_t k) {
+        const uint32_t n = shared().count, t = threadIdx.x;
+        if (n <= THIN) return;
+        if (t < 64) {
+            constexpr int W = (LIST + 63) / 64;
+            uint64_t own[W];
+#pragma unroll
+            for (int i = 0; i < W; ++i) own[i] = i * 64 + t < n ? shared().list[i * 64 + t] : 0ull;
+            uint32_t limit = 0;
+            for (int bit = 31; bit >= LOW_BIT; --bit) {
+                const uint32_t next = limit | (1u << bit);
+                uint32_t reach = 0;
+#pragma unroll
+                for (int i = 0; i < W; ++i)
+                    if (i * 64 < (int)n) reach += (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64((uint32_t)(own[i] >> 32) >= next));
+                if (reach >= k) limit = next;
+                if (reach == k) break;
+            }
+            uint32_t at = 0;
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                const bool keep = (uint32_t)(own[i] >> 32) >= limit && i * 64 + t < n;
+                const uint64_t in_wave = __builtin_amdgcn_ballot_w64(keep);
+                if (keep) shared().list[at + (uint32_t)__builtin_popcountll(in_wave & ((1ull << t) - 1))] = own[i];
+                at += (uint32_t)__builtin_popcountll(in_wave);
+            }
+            if (t == 0) shared().count = at;
+        }
+        __syncthreads();
+    }
+    // The list holds all logits above -inf.  If these are n < k, it gets the first k - n masked ones too, which are among
+    // the slice's first k elements.  (9240 rows of 365, a few logits left, k = 63: 42 us; with select_exactly() 95.)
+    static __device__ __forceinline__ void fill_up(const RowSpan<T>& span, const Slice& s, uint32_t k) {
+        const uint32_t n = shared().count, t = threadIdx.x, there = s.e1 - s.e0 < k ? s.e1 - s.e0 : k;
+        if (n >= k) return;
+        if (t < 64) {
+            const bool masked = t < there && order_of(LogitVec<T>::load(span.row + s.e0 + t)) == kMaskedOrder;
+            const uint64_t in_wave = __builtin_amdgcn_ballot_w64(masked);
+            const uint32_t at = n + (uint32_t)__builtin_popcountll(in_wave & ((1ull << t) - 1));
+            if (masked && at < k) shared().list[at] = composite(kMaskedOrder, s.e0 + t);
+        }
+        __syncthreads();
+        if (t == 0) shared().count = there;
+        __syncthreads();
+    }
     // Leaves at least the k largest of the slice (all of them, if it has fewer) in the list, in any order, given
     // the threshold of the threads' largest logits.  look(least): meets the thread's vectors, every(least): the same for
     // any least, -inf among them; top: the thread's largest logit; nan: the row holds a NaN or +inf.
     template <typename F, typename E>
     static __device__ __forceinline__ void select(const RowSpan<T>& span, const Slice& s, uint32_t limit, bool exact, float top, bool nan,
                                            uint32_t k, F look, E every) {
-        if (!nan && !(exact && limit == 0x007fffffu)) {   // (-inf: a mask has left fewer than k logits)
-            const float least = limit <= 0x007fffffu ? -kInf : logit_of(limit);
-            if (limit <= 0x007fffffu) every(least);
+        if (!nan) {
+            const bool masked = exact && limit == kMaskedOrder;
+            const float least = masked ? -3.402823466e38f : limit <= kMaskedOrder ? -kInf : logit_of(limit);
+            if (limit <= kMaskedOrder && !masked) every(least);
             else if (top >= least) look(least);
             edge(span, s, least);
             sift(least);
-            if (!overflow()) return;
+            if (!overflow()) {
+                if (masked) fill_up(span, s, k);
+                return;
+            }
         }
         select_exactly(span, s, k, limit, exact && !nan);
     }
@@ -773,7 +836,20 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_held_kernel(LogprobPar
     held.load(span, s, t);
     named.load_logits(span, p.vocab);
     const bool any = t < s.v1 || s.edge >= 0;
-    auto publish = [&](float hi) { if (k) Top::publish(hi, any, k); };
+    auto part = [&](int i) {
+        constexpr int each = NV / Top::PER;
+        uint32_t order = 0;
+#pragma unroll
+        for (int u = 0; u < each; ++u)
+            if (s.v0 + (i * each + u) * THREADS + t < s.v1) {
+                float x[N];
+                LogitVec<T>::unpack(held.raw[i * each + u], x);
+                const uint32_t o = order_of(largest(x));
+                order = order > o ? order : o;
+            }
+        return order;
+    };
+    auto publish = [&](float hi) { if (k) Top::publish(hi, any, k, part); };
     auto met = [&](float) {
         if (k) Top::find(k);
         return 0.f;
@@ -795,6 +871,7 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_held_kernel(LogprobPar
         held.each(s, t, [&](const float (&x)[N], uint32_t base) { Top::scan(x, span.index(base + t), from); });
     };
     Top::select(span, s, limit, exact, r.top, r.sum != r.sum, k, look, every);
+    Top::thin_out(k);
     write_alternatives<THREADS>(p, row, Top::shared().list, Top::shared().count, r, l);
 }
 
@@ -1037,11 +1114,11 @@ __global__ __launch_bounds__(kSplitThreads, 8) void token_logprobs_split_kernel(
             uint32_t order = 0xffffffffu;
             if (t < w.parts) order = (uint32_t)(take((const uint64_t*)(records + t * w.record_bytes + 16) + r - 1) >> 32);
             order = over16(order, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
-            if (t % 16 == 0) Top::shared().words[t / 16] = order;
+            if (t % 16 == 0) Top::shared().at[t / 16] = order;
         }
         __syncthreads();
-        uint32_t limit = Top::shared().words[0];
-        for (int i = 1; i < 4; ++i) limit = limit < Top::shared().words[i] ? limit : Top::shared().words[i];
+        uint32_t limit = Top::shared().at[0];
+        for (int i = 1; i < 4; ++i) limit = limit < Top::shared().at[i] ? limit : Top::shared().at[i];
         for (uint32_t i = t; i < w.parts * k; i += THREADS) {
             const uint64_t c = take((const uint64_t*)(records + (i / k) * w.record_bytes + 16) + i % k);
             if ((uint32_t)(c >> 32) >= limit) Top::append((uint32_t)(c >> 32), ~(uint32_t)c);
