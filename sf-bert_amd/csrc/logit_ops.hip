@@ -464,13 +464,14 @@ template <typename T, int THREADS, int HELD> struct TopSelect {
     static constexpr int PER = HELD >= 4 && THREADS < 256 ? 256 / THREADS : 1;
     static constexpr int GROUPS = THREADS * PER < 256 ? THREADS * PER : 256;
     static constexpr uint32_t THIN = 128;
+    static constexpr uint32_t kBetween = 0, kExact = 1, kCommon = 2;
     static constexpr int LOW_BIT = sizeof(T) == 2 ? 16 : 0;   // bf16 logits are told apart by the upper half
     static_assert(GROUPS <= VECTORS, "the groups share memory with the vectors");
     struct Shared {
         u32x4 vectors[VECTORS];       // vectors that hold a logit above the threshold
         uint64_t list[LIST];          // composites
         uint32_t at[VECTORS];         // index of each vector's first element; before: the groups' largest logits
-        uint32_t limit, exact;        // the threshold, and whether it is one of those
+        uint32_t limit, kind;         // the threshold
         uint32_t count, n_vectors;
     };
     static __device__ __forceinline__ Shared& shared() {
@@ -489,27 +490,37 @@ template <typename T, int THREADS, int HELD> struct TopSelect {
     }
 
     // The largest value that at least k of 64 * W groups' largest logits reach, found bit by bit by one wave; it ends
-    // early where exactly k reach it (*all: it did not, the threshold is one of them).
-    template <int W> static __device__ __forceinline__ uint32_t search(uint32_t k, uint32_t* all) {
+    // early where exactly k reach it (*kind = kBetween: the threshold need not be one of them).  kExact: it is one;
+    // kCommon: it is that of half of the groups, which is what a mask leaves (or rows of few different values).
+    template <int W> static __device__ __forceinline__ uint32_t search(uint32_t k, uint32_t* kind) {
         uint32_t own[W], limit = 0;
 #pragma unroll
         for (int i = 0; i < W; ++i) own[i] = shared().at[i * 64 + (threadIdx.x & 63)];
-        *all = 1;
+        *kind = kExact;
         for (int bit = 31; bit >= LOW_BIT; --bit) {
             const uint32_t next = limit | (1u << bit);
             uint32_t n = 0;
 #pragma unroll
             for (int i = 0; i < W; ++i) n += (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(own[i] >= next));
             if (n >= k) limit = next;
-            if (n == k) { *all = 0; break; }
+            if (n == k) { *kind = kBetween; break; }
         }
         // (orders of negative bf16 logits end in ones)
         if (LOW_BIT && !(limit >> 31)) limit |= (1u << LOW_BIT) - 1;
+        if (*kind == kExact && limit >= kMaskedOrder) {
+            uint32_t n = 0, there = 0;
+#pragma unroll
+            for (int i = 0; i < W; ++i) {
+                n += (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(own[i] == limit));
+                there += (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(own[i] != 0));
+            }
+            if (2 * n >= there) *kind = kCommon;
+        }
         return limit;
     }
     // A threshold that at least k logits of the threads' largest reach, in three parts with a barrier after the first and
     // the second: every thread publishes its largest logit (and count is cleared), one wave searches, all read the
-    // result; *exact: it is one of those logits.  Up to k = 32 the threads form 64 groups (k = 20: 24 logits expected
+    // result.  Up to k = 32 the threads form 64 groups (k = 20: 24 logits expected
     // above the threshold), beyond that up to 256; own(i): order of the i-th of this thread's PER groups.
     template <typename F> static __device__ __forceinline__ void publish(float top, bool any, uint32_t k, F own) {
         const uint32_t t = threadIdx.x;
@@ -531,21 +542,21 @@ template <typename T, int THREADS, int HELD> struct TopSelect {
     }
     static __device__ __forceinline__ void find(uint32_t k) {
         if (threadIdx.x >= 64) return;
-        uint32_t all;
-        const uint32_t limit = GROUPS > 64 && k > 32 ? search<GROUPS / 64>(k, &all) : search<1>(k, &all);
-        if (threadIdx.x == 0) { shared().limit = limit; shared().exact = all; }
+        uint32_t kind;
+        const uint32_t limit = GROUPS > 64 && k > 32 ? search<GROUPS / 64>(k, &kind) : search<1>(k, &kind);
+        if (threadIdx.x == 0) { shared().limit = limit; shared().kind = kind; }
     }
-    static __device__ __forceinline__ uint32_t found(bool* exact) {
-        *exact = shared().exact != 0;
+    static __device__ __forceinline__ uint32_t found(uint32_t* kind) {
+        *kind = shared().kind;
         return shared().limit;
     }
-    static __device__ __forceinline__ uint32_t threshold(float top, bool any, uint32_t k, bool* exact) {
+    static __device__ __forceinline__ uint32_t threshold(float top, bool any, uint32_t k, uint32_t* kind) {
         __syncthreads();
         publish(top, any, k, [](int) { return 0u; });
         __syncthreads();
         find(k);
         __syncthreads();
-        return found(exact);
+        return found(kind);
     }
     template <int CTRL> static __device__ __forceinline__ uint32_t pair_max(uint32_t v, bool take) {
         const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
@@ -599,7 +610,14 @@ template <typename T, int THREADS, int HELD> struct TopSelect {
             return true;
         });
         __syncthreads();
-        const uint32_t t = threadIdx.x, lane = t & 63, above = shared().count, want = k - above;
+        fill_up(span, s, k, limit);
+    }
+    // The list holds the logits above `limit`, which has no more than k - 1 above it: the lowest-index ones that equal it
+    // (behind a mask, among the slice's first ones) complete it to k, as far as there are any.
+    static __device__ void fill_up(const RowSpan<T>& span, const Slice& s, uint32_t k, uint32_t limit) {
+        const uint32_t t = threadIdx.x, lane = t & 63, above = shared().count;
+        if (above >= k) return;
+        const uint32_t want = k - above;
         uint32_t have = 0;
         elements(span, s, [&](uint32_t order, uint32_t j) {
             const bool equal = j < s.e1 && order == limit;
@@ -616,7 +634,7 @@ template <typename T, int THREADS, int HELD> struct TopSelect {
             return have < want;
         });
         __syncthreads();
-        if (t == 0) shared().count = k;
+        if (t == 0) shared().count = above + (have < want ? have : want);
         __syncthreads();
     }
 
@@ -650,10 +668,13 @@ template <typename T, int THREADS, int HELD> struct TopSelect {
     static __device__ __forceinline__ bool overflow() { return shared().n_vectors > (uint32_t)VECTORS || shared().count > (uint32_t)LIST; }
     // A long row's k largest are collected while it is read: a threshold from the threads' first vectors holds for the
     // whole row and lets through about as many times k logits as the row is longer than they are.
-    // The value from which logits are let through; NaN, which lets none through, where there are no k logits above -inf.
-    static __device__ __forceinline__ float early(float top, bool any, uint32_t k) {
-        bool exact;
-        const uint32_t limit = threshold(top, any, k, &exact);
+    // The value from which logits are let through; NaN, which lets none through, where there are no k logits.  *tie: the
+    // threshold itself, if only logits above it are let through (0: those that equal it too).
+    static __device__ __forceinline__ float early(float top, bool any, uint32_t k, uint32_t* tie) {
+        uint32_t kind;
+        const uint32_t limit = threshold(top, any, k, &kind);
+        *tie = kind == kCommon ? limit : 0u;
+        if (kind == kCommon) return logit_of(limit + 1);
         return limit <= kMaskedOrder ? __builtin_nanf("") : logit_of(limit);
     }
 
@@ -695,40 +716,27 @@ template <typename T, int THREADS, int HELD> struct TopSelect {
         }
         __syncthreads();
     }
-    // The list holds all logits above -inf.  If these are n < k, it gets the first k - n masked ones too, which are among
-    // the slice's first k elements.  (9240 rows of 365, a few logits left, k = 63: 42 us; with select_exactly() 95.)
-    static __device__ __forceinline__ void fill_up(const RowSpan<T>& span, const Slice& s, uint32_t k) {
-        const uint32_t n = shared().count, t = threadIdx.x, there = s.e1 - s.e0 < k ? s.e1 - s.e0 : k;
-        if (n >= k) return;
-        if (t < 64) {
-            const bool masked = t < there && order_of(LogitVec<T>::load(span.row + s.e0 + t)) == kMaskedOrder;
-            const uint64_t in_wave = __builtin_amdgcn_ballot_w64(masked);
-            const uint32_t at = n + (uint32_t)__builtin_popcountll(in_wave & ((1ull << t) - 1));
-            if (masked && at < k) shared().list[at] = composite(kMaskedOrder, s.e0 + t);
-        }
-        __syncthreads();
-        if (t == 0) shared().count = there;
-        __syncthreads();
-    }
     // Leaves at least the k largest of the slice (all of them, if it has fewer) in the list, in any order, given
     // the threshold of the threads' largest logits.  look(least): meets the thread's vectors, every(least): the same for
     // any least, -inf among them; top: the thread's largest logit; nan: the row holds a NaN or +inf.
+    // A mask's value would fill the list: only logits above it are collected then, and it is filled up.  (10 logits left,
+    // fp32, k = 20: 2000 rows of 131072 take 160 us, took 945 us with select_exactly(); 4096 rows of 30522 78 and 405.)
     template <typename F, typename E>
-    static __device__ __forceinline__ void select(const RowSpan<T>& span, const Slice& s, uint32_t limit, bool exact, float top, bool nan,
+    static __device__ __forceinline__ void select(const RowSpan<T>& span, const Slice& s, uint32_t limit, uint32_t kind, float top, bool nan,
                                            uint32_t k, F look, E every) {
         if (!nan) {
-            const bool masked = exact && limit == kMaskedOrder;
-            const float least = masked ? -3.402823466e38f : limit <= kMaskedOrder ? -kInf : logit_of(limit);
-            if (limit <= kMaskedOrder && !masked) every(least);
+            const bool above = kind == kCommon || (kind == kExact && limit == kMaskedOrder);
+            const float least = above ? logit_of(limit + 1) : limit <= kMaskedOrder ? -kInf : logit_of(limit);
+            if (least == -kInf) every(least);
             else if (top >= least) look(least);
             edge(span, s, least);
             sift(least);
             if (!overflow()) {
-                if (masked) fill_up(span, s, k);
+                if (above) fill_up(span, s, k, limit);
                 return;
             }
         }
-        select_exactly(span, s, k, limit, exact && !nan);
+        select_exactly(span, s, k, limit, kind != kBetween && !nan);
     }
 };
 
@@ -860,8 +868,8 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_held_kernel(LogprobPar
     named.write(p.logprob + row * p.n_tokens, p.n_tokens, r.m, l, p.scale);
     if (k == 0) return;
     if (THREADS == 64) __syncthreads();
-    bool exact;
-    const uint32_t limit = Top::found(&exact);
+    uint32_t kind;
+    const uint32_t limit = Top::found(&kind);
     auto look = [&](float from) {
         held.template steps<false>(s, t, [&](auto count, const u32x4* raw, uint32_t base) {
             Top::template meet<decltype(count)::value>(span, raw, largest_of<T, decltype(count)::value>(raw), base, from);
@@ -870,7 +878,7 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_held_kernel(LogprobPar
     auto every = [&](float from) {
         held.each(s, t, [&](const float (&x)[N], uint32_t base) { Top::scan(x, span.index(base + t), from); });
     };
-    Top::select(span, s, limit, exact, r.top, r.sum != r.sum, k, look, every);
+    Top::select(span, s, limit, kind, r.top, r.sum != r.sum, k, look, every);
     Top::thin_out(k);
     write_alternatives<THREADS>(p, row, Top::shared().list, Top::shared().count, r, l);
 }
@@ -878,10 +886,11 @@ __global__ __launch_bounds__(THREADS) void token_logprobs_held_kernel(LogprobPar
 // The sums of a streamed slice; with k > 0 its logits from `least` on are collected on the way.
 template <typename T, int THREADS, bool ENTROPY>
 __device__ __forceinline__ RowSum sum_and_collect(const RowSpan<T>& span, const Slice& s, float c, float* red, uint32_t k, bool any,
-                                                  float& least) {
+                                                  float& least, uint32_t& tie) {
     typedef TopSelect<T, THREADS, 0> Top;
     least = __builtin_nanf("");
-    auto early = [&](auto first) { if (k) least = Top::early(first(), any, k); };
+    tie = 0;
+    auto early = [&](auto first) { if (k) least = Top::early(first(), any, k, &tie); };
     auto meet = [&](auto count, const u32x4* raw, float hi, uint32_t base) {
         Top::template meet<decltype(count)::value>(span, raw, hi, base, least);
     };
@@ -889,20 +898,24 @@ __device__ __forceinline__ RowSum sum_and_collect(const RowSpan<T>& span, const 
 }
 // At least the k largest in the list.  Where the early threshold let too many through, or none, the row is read again.
 template <typename T, int THREADS>
-__device__ __forceinline__ void finish_collection(const RowSpan<T>& span, const Slice& s, const RowSum& r, uint32_t k, bool any, float least) {
+__device__ __forceinline__ void finish_collection(const RowSpan<T>& span, const Slice& s, const RowSum& r, uint32_t k, bool any, float least,
+                                                  uint32_t tie) {
     typedef TopSelect<T, THREADS, 0> Top;
     constexpr int N = LogitVec<T>::N;
     const uint32_t t = threadIdx.x;
     const bool nan = r.sum != r.sum;
     if (least == least) Top::edge(span, s, least);
     Top::sift(least);
-    if (least == least && !nan && !Top::overflow()) return;
-    bool exact = false;
-    const uint32_t limit = nan ? 0u : Top::threshold(r.top, any, k, &exact);
+    if (least == least && !nan && !Top::overflow()) {
+        if (tie) Top::fill_up(span, s, k, tie);
+        return;
+    }
+    uint32_t kind = Top::kBetween;
+    const uint32_t limit = nan ? 0u : Top::threshold(r.top, any, k, &kind);
     auto every = [&](float from) {
         Streamed<T, THREADS>::each(span, s, t, [&](const float (&x)[N], uint32_t base) { Top::scan(x, span.index(base + t), from); });
     };
-    Top::select(span, s, limit, exact, r.top, nan, k, every, every);
+    Top::select(span, s, limit, kind, r.top, nan, k, every, every);
 }
 
 // Long rows: one work-group per row, streamed.
@@ -919,12 +932,13 @@ __global__ __launch_bounds__(THREADS, 8) void token_logprobs_stream_kernel(Logpr
     named.load_logits(span, p.vocab);
     const bool any = t < s.v1 || s.edge >= 0;
     float least;
-    const RowSum r = sum_and_collect<T, THREADS, ENTROPY>(span, s, p.c, red, k, any, least);
+    uint32_t tie;
+    const RowSum r = sum_and_collect<T, THREADS, ENTROPY>(span, s, p.c, red, k, any, least, tie);
     const float l = log2f(r.sum);
     if (t == 0) write_row_sums<ENTROPY>(p, row, r, l);
     named.write(p.logprob + row * p.n_tokens, p.n_tokens, r.m, l, p.scale);
     if (k == 0) return;
-    finish_collection<T, THREADS>(span, s, r, k, any, least);
+    finish_collection<T, THREADS>(span, s, r, k, any, least, tie);
     write_alternatives<THREADS>(p, row, Top::shared().list, Top::shared().count, r, l);
 }
 
@@ -1092,12 +1106,13 @@ __global__ __launch_bounds__(kSplitThreads, 8) void token_logprobs_split_kernel(
     named.load_logits(span, p.vocab);
     const bool any = s.v0 + t < s.v1 || s.edge >= 0;
     float least;
-    RowSum r = sum_and_collect<T, THREADS, ENTROPY>(span, s, p.c, red, k, any, least);
+    uint32_t tie;
+    RowSum r = sum_and_collect<T, THREADS, ENTROPY>(span, s, p.c, red, k, any, least, tie);
     uint8_t* const records = w.records + row * w.parts * w.record_bytes;
     uint8_t* const record = records + part * w.record_bytes;
     if (t < 3) leave((float*)record + t, t == 0 ? r.m : t == 1 ? r.sum : r.dot);
     if (k) {
-        finish_collection<T, THREADS>(span, s, r, k, any, least);
+        finish_collection<T, THREADS>(span, s, r, k, any, least, tie);
         const uint32_t n = Top::shared().count;
         uint64_t* const best = (uint64_t*)(record + 16);
         ranked<THREADS>(Top::shared().list, n, k, [&](uint32_t rank, uint64_t c) { leave(best + rank, c); });

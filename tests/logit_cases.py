@@ -21,6 +21,7 @@ def round_bf16(x):
 
 KINDS = ["normal", "peaked", "ties", "masked", "lowest", "all lowest", "rising", "empty", "huge", "constant", "nan", "inf",
          "zeros", "late peak"]
+MASKS_AND_TIES = ["spread ties", "late ties", "open half", "open half, lowest", "ten left", "ten and masked", "masked"]
 
 
 def logits_of(kind, vocab, rng, bf16):
@@ -54,6 +55,26 @@ def logits_of(kind, vocab, rng, bf16):
         x = np.where(rng.random(vocab) < 0.5, np.float32(0.0), np.float32(-0.0))
     elif kind == "late peak":
         x[-1] = 30.0
+    elif kind == "spread ties":   # the largest but for two is one value all over the row
+        x *= 0.1
+        x[5::37] = 7.0
+        x[rng.integers(0, vocab, 2)] = 9.0
+    elif kind == "late ties":     # and at its end
+        x *= 0.1
+        x[vocab // 8 * 7:] = 7.0
+    elif kind == "open half":     # nothing but masked logits in the first half
+        x[:vocab // 2] = -np.inf
+    elif kind == "open half, lowest":
+        x[:vocab // 2] = LOWEST[True]
+    elif kind == "ten left":
+        keep = rng.integers(0, vocab, 10)
+        x, kept = np.full(vocab, LOWEST[True], np.float32), x[keep]
+        x[keep] = kept
+    elif kind == "ten and masked":   # masked logits of two kinds
+        keep = rng.integers(0, vocab, 10)
+        x, kept = np.full(vocab, LOWEST[True], np.float32), x[keep]
+        x[::3] = -np.inf
+        x[keep] = kept
     return round_bf16(x) if bf16 else x.astype(np.float32)
 
 

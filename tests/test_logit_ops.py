@@ -85,6 +85,16 @@ def test_few_tokens_named_many_times_on_the_device(vocab, bf16):
         cases.distillation(*device_backend(), vocab, bf16, 1, slots=n, few=True, seed=71 + n)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab,bf16", [(70, False), (365, False), (1000, True), (2000, False), (3500, False), (9001, True), (30522, False), (140001, True)])
+def test_alternatives_behind_masks_and_among_ties_on_the_device(vocab, bf16):
+    S, dev = device_backend()
+    ws = torch.zeros(S.LOGIT_WORKSPACE_BYTES, dtype=torch.uint8, device="cuda")
+    for k in (1, 20, 33, 64):
+        cases.logprobs(S, dev, vocab, bf16, 0, n=1, k=k, kinds=cases.MASKS_AND_TIES, seed=90 + k)
+        cases.logprobs(S, dev, vocab, bf16, 3, n=1, k=k, kinds=cases.MASKS_AND_TIES, seed=91 + k, workspace=ws, repeat=2)
+
+
 FAR_APART = [(11, False), (200, True), (1000, False), (2500, False), (9001, True), (40000, False)]
 
 
@@ -288,6 +298,15 @@ def test_few_tokens_named_many_times_on_the_host_model(E, vocab, bf16, order):  
     for n in (2, 67):
         cases.logprobs_backward(*back, vocab, bf16, 0, n=n, few=True, seed=70 + n, kinds=some)
         cases.distillation(*back, vocab, bf16, 1, slots=n, few=True, seed=71 + n, kinds=some)
+
+
+@pytest.mark.parametrize("vocab,bf16,order", [(70, False, 0), (365, False, 1), (2000, False, 14), (3500, False, 0), (9001, True, 21)])
+def test_alternatives_behind_masks_and_among_ties_on_the_host_model(E, vocab, bf16, order):   # noqa: F811
+    S, dev = host_backend(E, order=order)
+    ws = dev(np.zeros(S.LOGIT_WORKSPACE_BYTES, np.uint8))
+    for k in (20, 64):
+        cases.logprobs(S, dev, vocab, bf16, 3, n=1, k=k, kinds=cases.MASKS_AND_TIES, seed=90 + k)
+        cases.logprobs(S, dev, vocab, bf16, 0, n=1, k=k, kinds=cases.MASKS_AND_TIES, seed=91 + k, workspace=ws)
 
 
 @pytest.mark.parametrize("vocab,bf16", FAR_APART[:-1])
