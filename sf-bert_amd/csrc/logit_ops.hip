@@ -5,6 +5,9 @@
 // With s = scale, c = s log2(e), a row x and any reference m:  S = sum_j 2^((x_j - m) c),  l = log2 S,
 //   ln p_j = (x_j - m) s - ln2 l,   entropy = ln2 (l - W / S) with W = sum_j 2^t_j t_j, t_j = (x_j - m) c.
 // Everything is held in fp32.  The row is read once; (m, l) is what the backward pass is given.
+//
+// What bounds these kernels is reading the rows (and writing gradients): this card reads 7.1 TB/s and copies 6.2 with
+// nontemporal accesses, 6.3 and 5.6 with plain ones, so every row's vectors are loaded and stored nontemporally.
 #include "common.hip.h"
 
 namespace sfb {
@@ -460,7 +463,7 @@ template <typename T, int THREADS, int HELD> struct TopSelect {
     static constexpr int VECTORS = HELD && HELD * THREADS < 256 ? HELD * THREADS : 256;
     static constexpr int LIST = HELD && HELD * THREADS * N + 16 < 512 ? HELD * THREADS * N + 16 : 512;
     // (one or two waves that hold a row give several groups each thread: with 64 groups and 64 alternatives the
-    // threshold is the least of the threads' maxima, 8000 rows of 2000 took 880 us for 25)
+    // threshold is the least of the threads' maxima: 8000 rows of 2000 took 880 us, take 36)
     static constexpr int PER = HELD >= 4 && THREADS < 256 ? 256 / THREADS : 1;
     static constexpr int GROUPS = THREADS * PER < 256 ? THREADS * PER : 256;
     static constexpr uint32_t THIN = 128;
@@ -685,7 +688,8 @@ template <typename T, int THREADS, int HELD> struct TopSelect {
         }
     }
     // Few threads and many alternatives: the threshold lets most of a row through, and ranking n logits costs n^2.  One
-    // wave finds the k-th largest of the list and keeps those that reach it.
+    // wave finds the k-th largest of the list and keeps those that reach it.  (9240 rows of 365 with 63: 36 us, without
+    // this 97.)
     static __device__ __forceinline__ void thin_out(uint32_t k) {
         const uint32_t n = shared().count, t = threadIdx.x;
         if (n <= THIN) return;
@@ -828,7 +832,10 @@ template <int THREADS> __device__ __forceinline__ void write_alternatives(const 
     });
 }
 
-// Short rows: one work-group per row, held in registers (NV vectors per thread).
+// Short rows: one work-group per row, held in registers (NV vectors per thread), so that the sums are taken relative to
+// the row's maximum and the alternatives are looked up without another read.  8192 rows of 2000 fp32 logits with entropy
+// take 14.8 us (4.4 TB/s), with 4 alternatives 19.6; with tens of them the instructions of their search count for more
+// than the memory (8000 rows, 64 alternatives: 36 us).
 template <typename T, int THREADS, int NV, bool ENTROPY>
 __global__ __launch_bounds__(THREADS) void token_logprobs_held_kernel(LogprobParams p) {
     typedef TopSelect<T, THREADS, NV> Top;
@@ -918,7 +925,9 @@ __device__ __forceinline__ void finish_collection(const RowSpan<T>& span, const 
     Top::select(span, s, limit, kind, r.top, nan, k, every, every);
 }
 
-// Long rows: one work-group per row, streamed.
+// Long rows: one work-group per row, streamed.  8192 rows of 50257 bf16 logits take 126 us (6.5 TB/s), 4096 of 30522 fp32
+// with entropy and 5 alternatives 80 us (6.3 TB/s): bound by memory.  With entropy, bf16 rows are bound by instructions
+// nearly as much: 4096 of 30522 take 43 us (5.8 TB/s), 53 with 20 alternatives.
 template <typename T, int THREADS, bool ENTROPY>
 __global__ __launch_bounds__(THREADS, 8) void token_logprobs_stream_kernel(LogprobParams p) {
     typedef TopSelect<T, THREADS, 0> Top;
@@ -943,7 +952,9 @@ __global__ __launch_bounds__(THREADS, 8) void token_logprobs_stream_kernel(Logpr
 }
 
 // Very short rows: 16 lanes a row, so that a wave's instructions serve four rows and every reduction is four DPP moves.
-// Up to kShortTop alternatives are taken out one by one.
+// Up to kShortTop alternatives are taken out one by one, which is what bounds this kernel: 32768 rows of 256 fp32 logits
+// take 7.6 us without alternatives (4.5 TB/s) and 14.8 with 4, where a wave for each row takes 14.0 and 24.7.  (8
+// alternatives: 20.8 and 24.7; more are left to those.  500 bf16 logits: 21 and 32.)
 constexpr uint32_t kShortTop = 8, kShortVecs = 64, kShortRows = 16;
 
 template <int CTRL> __device__ __forceinline__ uint32_t dpp(uint32_t v) {
@@ -1039,7 +1050,8 @@ __global__ __launch_bounds__(256) void token_logprobs_short_kernel(LogprobParams
 // Each row is cut into parts with a work-group each.  A part leaves its sums and its own k largest in the workspace; the
 // one that arrives last joins them (in the order of the parts) and writes the row, and clears the row's counter.  Records
 // go through the memory system's coherent level with device-scope stores and loads; a part waits for its stores before
-// it counts itself as arrived.
+// it counts itself as arrived.  Bound by latency: one row of 30522 fp32 logits with 5 alternatives takes 8.4 us, 48 of
+// 131072 bf16 with 20 13 us (27 by one work-group a row).
 constexpr uint32_t kSplitRows = 512, kSplitParts = 64, kSplitThreads = 512;
 
 struct SplitWork {
@@ -1090,7 +1102,7 @@ __device__ __forceinline__ void join_sums(const SplitWork& w, size_t row, const 
 }
 
 template <typename T, bool ENTROPY>
-__global__ __launch_bounds__(kSplitThreads, 8) void token_logprobs_split_kernel(LogprobParams p, SplitWork w) {
+__global__ __launch_bounds__(kSplitThreads, 4) void token_logprobs_split_kernel(LogprobParams p, SplitWork w) {
     constexpr int THREADS = kSplitThreads;
     typedef TopSelect<T, THREADS, 0> Top;
     typedef Streamed<T, THREADS> Stream;
@@ -1173,7 +1185,7 @@ struct RowGrad {
 // The tokens that a row's coefficients belong to, and those coefficients, in shared memory, filled up with id -1 to a
 // whole number of fours.  Tokens named more than once are rare but have to add up: a bit per token (its lower 13 bits)
 // tells the slots that come second to one, and only tokens that such a slot names are searched for in the whole list.
-// (Every slot searching cost ten times the row itself at 3339 logits and 150 slots.)
+// (5801 bf16 rows of 3339 logits and 150 slots: 22 us, 58 with every slot searching.)
 struct Slots {
     int32_t id[kMaxSlots];
     float coef[kMaxSlots];
@@ -1343,9 +1355,10 @@ struct GradParams {
     float scale, c;
 };
 
+// One work-group per THREADS * kGradVecs vectors of a row, all read before the first is written.  Bound by memory: 2048
+// rows of 50257 fp32 logits against a teacher's 100 take 139 us (5.9 TB/s read and written), 4096 of 30522 bf16 with the
+// entropy's term 93 us (5.4 TB/s).  Pieces of 1024 to 4096 vectors differ by a few percent.
 constexpr int kGradVecs = 4;
-
-// One work-group per THREADS * kGradVecs vectors of a row.
 template <typename T, int THREADS, bool ENTROPY, bool TEACHER>
 __global__ __launch_bounds__(THREADS) void logit_gradient_kernel(GradParams p) {
     constexpr int NV = kGradVecs;
@@ -1443,8 +1456,11 @@ __device__ __forceinline__ float row_loss(const Teacher& teacher, float l, float
 // and (GRAD) the gradient, for which a held row is not read again.  The teacher's softmax and the logits of its tokens
 // are ready by the time the row has arrived; with m, l of the student and q of the teacher the loss is
 //   ( sum q ln q + ln2 l ) / s^2 - sum q (x - m) / s.
+// With the gradient it reads and writes every logit once, which is what bounds it: 8192 rows of 30522 bf16 logits take
+// 185 us (5.4 TB/s), 4096 of 131072 416 us (5.2 TB/s), where a copy reaches 6.2: a compute unit has registers for four
+// such rows (one of the long ones), and neither reads nor writes for a row that is between its sums and its gradient.
 template <typename T, int THREADS, int NV, bool GRAD>
-__global__ __launch_bounds__(THREADS, THREADS == 1024 && NV == 8 ? 8 : 4) void distill_kernel(DistillParams p) {
+__global__ __launch_bounds__(THREADS, 4) void distill_kernel(DistillParams p) {
     __shared__ float red[2 * THREADS / 64];
     __shared__ Slots slots;
     __shared__ uint32_t some_teacher;
@@ -1580,7 +1596,13 @@ template <typename T> __global__ __launch_bounds__(kSplitThreads, 8) void distil
     }
 }
 
-// How a row is spread over a work-group: threads, and vectors per thread held in registers (0: streamed).
+// How a row is spread over a work-group: threads, and vectors per thread held in registers (0: streamed).  Fewer threads
+// wait less for each other, as long as enough rows fit a compute unit.  8192 bf16 rows with their gradient, us: 2000
+// logits 20 at {64, 4} and 33 at {256, 4}; 4000: 30 at {64, 8}, 31 at {128, 8}, 33 at {256, 4}; 6000: 43 at {128, 8}, 45
+// at {256, 4}; 16000: 99 at {256, 8}, 107 at {512, 8}, 154 at {1024, 8}; 30522: 188 at {512, 8}, 196 at {256, 16}.  4096
+// rows of 64000: 186 at {512, 16}, 192 at {1024, 8}, 231 at {1024, 12}, 259 at {1024, 0}, where the row is read twice; of
+// 96000: 288 at {512, 24}, 321 at {1024, 12}; of 131072: 418 at {1024, 16}, 423 at {512, 32}.
+// Without the gradient nothing needs to be kept, and long rows are streamed.
 struct RowShape { int threads, vecs; };
 static inline RowShape distill_shape(uint32_t vocab, int dtype, bool gradient) {
     const uint32_t vecs = vocab / (dtype == SFB_BF16 ? 8u : 4u);
@@ -1591,8 +1613,8 @@ static inline RowShape distill_shape(uint32_t vocab, int dtype, bool gradient) {
     if (!gradient) return {512, 0};
     if (vecs <= 2048) return {256, 8};
     if (vecs <= 4096) return {512, 8};
-    if (vecs <= 8192) return {1024, 8};
-    if (vecs <= 12288) return {1024, 12};
+    if (vecs <= 8192) return {512, 16};
+    if (vecs <= 12288) return {512, 24};
     if (vecs <= 16384) return {1024, 16};
     return {1024, 0};
 }
@@ -1661,6 +1683,11 @@ extern "C" int sfb_token_logprobs(sfb_stream_t stream, float* logprob, float* en
     clear_stale_error();
     const uint32_t vecs = vocab / (dtype == SFB_BF16 ? 8u : 4u);
     const SplitWork w = split_rows(workspace, rows, vecs, top_k, 256);
+    // Rows that one or two waves hold, else streamed.  8192 fp32 rows with 4 alternatives, us: 1000 logits 14 at 64 x 4, 23
+    // at 256 x 4, 43 streamed by 512 threads; 2000: 20 at 64 x 8 and at 128 x 8, 25 at 256 x 4; 4000: 29 at 128 x 8, 32 at
+    // 256 x 4, 33 streamed by 256 threads, 49 by 512.  Alternatives of streamed rows cost less with fewer threads until
+    // the rows are long: 4096 bf16 rows of 30522 with 20 53 by 256 threads and 58 by 512, without 45 and 44; 4096 fp32
+    // ones 89 and 85.
     const bool is_short = vecs <= kShortVecs && top_k <= kShortTop;
     if (too_many(rows, is_short ? 256 / kShortRows : vecs <= 512 ? 64 : vecs <= 1024 ? 128 : 512)) return SFB_ERR_SHAPE;
     const dim3 grid((uint32_t)rows);
@@ -1691,6 +1718,7 @@ extern "C" int sfb_token_logprobs(sfb_stream_t stream, float* logprob, float* en
 
 static int launch_gradient(hipStream_t s, GradParams& p, int dtype, uint64_t rows, bool entropy, bool teacher) {
     const uint32_t vecs = p.vocab / (dtype == SFB_BF16 ? 8u : 4u);
+    // (a row by one wave: 15347 rows of 833 fp32 logits, loss and gradient, 35 us; 50 by four.  8000 of 1500: 38 and 36)
     const uint32_t threads = vecs <= 256 ? 64 : 256;
     p.each = threads * kGradVecs;
     p.parts = vecs == 0 ? 1 : (vecs + p.each - 1) / p.each;
@@ -1775,9 +1803,9 @@ extern "C" int sfb_distillation_loss(sfb_stream_t stream, float* row_loss, float
         else if (shape.threads == 128) distill_kernel<T, 128, 8, GRAD><<<grid, 128, 0, s>>>(p);                    \
         else if (!GRAD) distill_kernel<T, 512, 0, false><<<grid, 512, 0, s>>>(p);                                  \
         else if (shape.threads == 256) distill_kernel<T, 256, 8, true><<<grid, 256, 0, s>>>(p);                    \
-        else if (shape.threads == 512) distill_kernel<T, 512, 8, true><<<grid, 512, 0, s>>>(p);                    \
-        else if (shape.vecs == 8) distill_kernel<T, 1024, 8, true><<<grid, 1024, 0, s>>>(p);                       \
-        else if (shape.vecs == 12) distill_kernel<T, 1024, 12, true><<<grid, 1024, 0, s>>>(p);                     \
+        else if (shape.vecs == 8) distill_kernel<T, 512, 8, true><<<grid, 512, 0, s>>>(p);                         \
+        else if (shape.threads == 512 && shape.vecs == 16) distill_kernel<T, 512, 16, true><<<grid, 512, 0, s>>>(p); \
+        else if (shape.vecs == 24) distill_kernel<T, 512, 24, true><<<grid, 512, 0, s>>>(p);                       \
         else if (shape.vecs == 16) distill_kernel<T, 1024, 16, true><<<grid, 1024, 0, s>>>(p);                     \
         else distill_kernel<T, 1024, 0, true><<<grid, 1024, 0, s>>>(p);                                            \
     } while (0)
