@@ -1620,13 +1620,17 @@ static inline RowShape distill_shape(uint32_t vocab, int dtype, bool gradient) {
 }
 
 // Parts of each row of a launch that would otherwise leave most of the device idle: about `groups` work-groups in all, of
-// at least 1024 vectors each.  (48 rows of 16384 vectors with 20 alternatives: 13 us as 240 groups, 15 as 480, 17 as 768,
-// 27 whole.)  parts = 0: no workspace, or too many rows.
+// at least 1024 vectors each, or up to 512 where rows would otherwise be halved at most and 8192 are left each.  With 20
+// alternatives, us: 48 rows of 16384 vectors 12.4 as 240 groups, 13.6 as 480, 15 as 720, 19.5 whole; 200 of 32768 27 as
+// 400, 45 whole; 100 of them 18 as 500, 22 as 200; 200 of 6282 15.6 as 400, 11.8 whole.  parts = 0: no workspace, or too
+// many rows.
 static inline SplitWork split_rows(void* workspace, uint64_t rows, uint32_t vecs, uint32_t k, uint32_t groups) {
     SplitWork w{};
     if (!workspace || rows > kSplitRows) return w;
     uint32_t parts = groups / (uint32_t)rows;
     if (parts > vecs / 1024) parts = vecs / 1024;
+    const uint32_t more = 512 / (uint32_t)rows, longer = vecs / 8192;
+    if (parts <= 2 && parts < more && parts < longer) parts = more < longer ? more : longer;
     if (parts > kSplitParts) parts = kSplitParts;
     if (k && parts > 512 / k) parts = 512 / k;   // (the parts' alternatives fit one list)
     if (parts < 1) parts = 1;
