@@ -3,7 +3,6 @@ alternatives, and the distillation loss against a teacher's top logits, each wit
 
 ``own`` False: the operators in elementary torch operations (fp32, rounded once at the end); True: the calls that a user
 makes of the package."""
-import functools
 import math
 
 import torch
@@ -190,8 +189,7 @@ def _plain_distill(s):
 
 
 # ---------------------------------------------------------------------------------------------- the package
-@functools.lru_cache(maxsize=None)
-def _package():   # a program imports it once
+def _package():
     import importlib
     return importlib.import_module("sf-bert_amd")
 
