@@ -431,6 +431,8 @@ template <typename T, int THREADS> struct Streamed {
             const float d = ref == top ? -rounding : (ref - top) * c - rounding, f = exp2_fast(d);
             if (ENTROPY) r.dot = f * (r.dot + fmaxf(d, -256.f) * r.sum);
             r.sum *= f;
+        } else {   // nothing near the row's largest logit: no share in the sums but a NaN's
+            r.sum = r.dot = r.sum == r.sum ? 0.f : r.sum;
         }
         r.m = top;
         if (EXTRA) r.dot = met(top == -kInf ? 0.f : top);

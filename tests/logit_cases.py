@@ -75,6 +75,10 @@ def logits_of(kind, vocab, rng, bf16):
         x, kept = np.full(vocab, LOWEST[True], np.float32), x[keep]
         x[::3] = -np.inf
         x[keep] = kept
+    elif kind.startswith("behind "):   # a mask of any value
+        keep = rng.integers(0, vocab, 10)
+        x, kept = np.full(vocab, float(kind[7:]), np.float32), x[keep]
+        x[keep] = kept
     return round_bf16(x) if bf16 else x.astype(np.float32)
 
 
@@ -418,6 +422,15 @@ def far_apart(S, dev, vocab, bf16, workspace=None):
             got = S.distillation_loss(t, dev(ids), dev(z), scale=scale, d_loss=d_loss, workspace=workspace)
             # (q's error: 5 u |t| + (slots + 40) u relative, |t| the teacher's largest exponent)
             same(host(got["row_loss"]), loss, U * (12 + 44 + 5 * 8 * scale) * np.abs(loss), "row_loss")
+
+
+def far_masks(S, dev, vocab, bf16, mask, scale, workspace=None):
+    """Masks that are neither -inf nor the type's lowest value, but far below the other logits: what is behind them has
+    probability 0."""
+    kinds = ["behind %r" % mask] * 2 + ["normal", "masked", "behind %r" % mask, "empty"]
+    logprobs(S, dev, vocab, bf16, 1, n=2, k=min(vocab, 12), scale=scale, workspace=workspace, kinds=kinds, seed=110)
+    logprobs(S, dev, vocab, bf16, 0, n=1, k=0, scale=scale, workspace=workspace, kinds=kinds, seed=111, entropy=False)
+    distillation(S, dev, vocab, bf16, 0, slots=6, scale=scale, workspace=workspace, kinds=kinds, seed=112)
 
 
 def refusals(S, dev):

@@ -106,6 +106,19 @@ def test_logits_far_apart_on_the_device(vocab, bf16):
     cases.far_apart(S, dev, vocab, bf16, workspace=torch.zeros(S.LOGIT_WORKSPACE_BYTES, dtype=torch.uint8, device="cuda"))
 
 
+# masks whose scaled value is -1e30 in fp32 (the products' factors are 1 and 10), or close to it
+FAR_MASKS = [(-1e30, float(np.float32(np.log(2.0)))), (-1e29, 6.931472)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mask,scale", FAR_MASKS)
+@pytest.mark.parametrize("vocab,bf16", [(300, True), (9001, False), (20000, True), (70001, False), (140001, True)])
+def test_far_masks_on_the_device(vocab, bf16, mask, scale):
+    S, dev = device_backend()
+    cases.far_masks(S, dev, vocab, bf16, mask, scale)
+    cases.far_masks(S, dev, vocab, bf16, mask, scale, workspace=torch.zeros(S.LOGIT_WORKSPACE_BYTES, dtype=torch.uint8, device="cuda"))
+
+
 @pytest.mark.gpu
 def test_teacher_to_student_on_the_device():
     cases.teacher_to_student(*device_backend())
@@ -314,6 +327,14 @@ def test_logits_far_apart_on_the_host_model(E, vocab, bf16):   # noqa: F811
     S, dev = host_backend(E)
     cases.far_apart(S, dev, vocab, bf16)
     cases.far_apart(S, dev, vocab, bf16, workspace=dev(np.zeros(S.LOGIT_WORKSPACE_BYTES, np.uint8)))
+
+
+@pytest.mark.parametrize("mask,scale", FAR_MASKS)
+@pytest.mark.parametrize("vocab,bf16", [(300, True), (3000, False), (9001, False), (20000, True)])
+def test_far_masks_on_the_host_model(E, vocab, bf16, mask, scale):   # noqa: F811
+    S, dev = host_backend(E)
+    cases.far_masks(S, dev, vocab, bf16, mask, scale)
+    cases.far_masks(S, dev, vocab, bf16, mask, scale, workspace=dev(np.zeros(S.LOGIT_WORKSPACE_BYTES, np.uint8)))
 
 
 def test_teacher_to_student_on_the_host_model(E):   # noqa: F811
