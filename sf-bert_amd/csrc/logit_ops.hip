@@ -16,10 +16,12 @@ constexpr uint32_t kMaxTop = 64;      // alternatives per row
 constexpr uint32_t kMaxSlots = 256;   // given tokens, or entries of a teacher's list, per row
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kInf = __builtin_inff();
-// Scaled reference (m c) of a lane that has not met a logit yet; logits whose scaled value passes kWide in either
-// direction are left to a second pass over the row that subtracts the maximum before it scales.
-constexpr float kNoReference = -1.0e30f;
-constexpr float kWide = 1.0e29f;
+// A reference's scaled value m c is rounded, and what rounding leaves out must stay a small exponent: up to kWide that is
+// at most one.  Rows whose largest scaled logit passes kWide in either direction are left to a second pass that subtracts
+// the maximum before it scales.  kNoReference: the scaled reference of a lane that has not met a logit above it yet; in
+// all other rows what stays below it is at least kWide powers of two from the largest logit.
+constexpr float kWide = 0x1p24f;
+constexpr float kNoReference = -0x1p25f;
 
 // A 16-byte vector of logits.
 template <typename T> struct LogitVec;
@@ -237,7 +239,7 @@ __device__ __forceinline__ void add_terms(const u32x4* raw, float c, float ref2,
     }
 }
 
-// Logits whose scaled values pass this in either direction are subtracted from the maximum before they are scaled.
+// Rows whose logits are subtracted from the maximum before they are scaled.
 __device__ __forceinline__ bool is_wide(float m, float c) { return fabsf(m * c) > kWide && fabsf(m) < kInf; }
 
 template <int V> struct Int { static constexpr int value = V; };

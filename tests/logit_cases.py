@@ -79,6 +79,10 @@ def logits_of(kind, vocab, rng, bf16):
         keep = rng.integers(0, vocab, 10)
         x, kept = np.full(vocab, float(kind[7:]), np.float32), x[keep]
         x[keep] = kept
+    elif kind.startswith("all of "):   # a row whose logits are all masked
+        x[:] = float(kind[7:])
+    elif kind.startswith("around "):   # neighbours among the numbers of that size
+        x = np.float32(float(kind[7:])) * (1 + rng.integers(0, 4, vocab) * np.float32(2.0 ** -7 if bf16 else 2.0 ** -23))
     return round_bf16(x) if bf16 else x.astype(np.float32)
 
 
@@ -431,6 +435,17 @@ def far_masks(S, dev, vocab, bf16, mask, scale, workspace=None):
     logprobs(S, dev, vocab, bf16, 1, n=2, k=min(vocab, 12), scale=scale, workspace=workspace, kinds=kinds, seed=110)
     logprobs(S, dev, vocab, bf16, 0, n=1, k=0, scale=scale, workspace=workspace, kinds=kinds, seed=111, entropy=False)
     distillation(S, dev, vocab, bf16, 0, slots=6, scale=scale, workspace=workspace, kinds=kinds, seed=112)
+
+
+def far_from_zero(S, dev, vocab, bf16, value, scale, workspace=None):
+    """Logits so far from zero that neighbouring scaled values are hundreds of powers of two apart, as a mask, as whole
+    rows and as the row's largest."""
+    kinds = ["behind %r" % value, "all of %r" % value, "normal", "around %r" % value, "masked", "all of %r" % value,
+             "behind %r" % value]
+    logprobs(S, dev, vocab, bf16, 1, n=2, k=min(vocab, 12), scale=scale, workspace=workspace, kinds=kinds, seed=120)
+    logprobs(S, dev, vocab, bf16, 0, n=1, k=0, scale=scale, workspace=workspace, kinds=kinds, seed=121, entropy=False)
+    logprobs_backward(S, dev, vocab, bf16, 0, n=2, scale=scale, kinds=kinds, seed=122)
+    distillation(S, dev, vocab, bf16, 0, slots=6, scale=scale, workspace=workspace, kinds=kinds, seed=123)
 
 
 def refusals(S, dev):

@@ -119,6 +119,18 @@ def test_far_masks_on_the_device(vocab, bf16, mask, scale):
     cases.far_masks(S, dev, vocab, bf16, mask, scale, workspace=torch.zeros(S.LOGIT_WORKSPACE_BYTES, dtype=torch.uint8, device="cuda"))
 
 
+FAR_FROM_ZERO = [(-1e10, 1.0), (-3e10, 0.7), (-1e20, 1.0), (-1e29, 1.0), (1e10, 1.0), (-2.0 ** 24, 1.0), (-3e7, 0.7), (-1e10, 1e-3)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("value,scale", FAR_FROM_ZERO)
+@pytest.mark.parametrize("vocab,bf16", [(200, False), (3000, False), (9001, False), (20000, True), (140001, True)])
+def test_logits_far_from_zero_on_the_device(vocab, bf16, value, scale):
+    S, dev = device_backend()
+    cases.far_from_zero(S, dev, vocab, bf16, value, scale)
+    cases.far_from_zero(S, dev, vocab, bf16, value, scale, workspace=torch.zeros(S.LOGIT_WORKSPACE_BYTES, dtype=torch.uint8, device="cuda"))
+
+
 @pytest.mark.gpu
 def test_teacher_to_student_on_the_device():
     cases.teacher_to_student(*device_backend())
@@ -335,6 +347,13 @@ def test_far_masks_on_the_host_model(E, vocab, bf16, mask, scale):   # noqa: F81
     S, dev = host_backend(E)
     cases.far_masks(S, dev, vocab, bf16, mask, scale)
     cases.far_masks(S, dev, vocab, bf16, mask, scale, workspace=dev(np.zeros(S.LOGIT_WORKSPACE_BYTES, np.uint8)))
+
+
+@pytest.mark.parametrize("value,scale", FAR_FROM_ZERO)
+@pytest.mark.parametrize("vocab,bf16", [(200, False), (3000, False), (9001, False), (20000, True)])
+def test_logits_far_from_zero_on_the_host_model(E, vocab, bf16, value, scale):   # noqa: F811
+    S, dev = host_backend(E)
+    cases.far_from_zero(S, dev, vocab, bf16, value, scale, workspace=dev(np.zeros(S.LOGIT_WORKSPACE_BYTES, np.uint8)) if vocab > 9000 else None)
 
 
 def test_teacher_to_student_on_the_host_model(E):   # noqa: F811
