@@ -697,6 +697,7 @@ template <typename T, int THREADS, int HELD> struct TopSelect {
     static __device__ __forceinline__ void thin_out(uint32_t k) {
         const uint32_t n = shared().count, t = threadIdx.x;
         if (n <= THIN) return;
+        if (THREADS > 64) __syncthreads();   // (all have read the count before the first wave writes it)
         if (t < 64) {
             constexpr int W = (LIST + 63) / 64;
             uint64_t own[W];

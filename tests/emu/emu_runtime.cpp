@@ -50,7 +50,8 @@ struct Block {
 };
 
 struct Config {
-    int order = 0;        // 0 ascending, 1 descending, n > 1: shuffled with seed n
+    int order = 0;        // 0 ascending, 1 descending, n > 1: shuffled with seed n, -1 - w: wave w runs as far as it can
+                          // before any other wave of its work-group moves
     int lazy_loads = 1;   // LDS-direct loads land at the wait (1) or when issued (0)
     int resident = 64;    // work-groups in flight at a time
     bool fixed = false;   // no further work-group is started for lanes that poll (a launch with more work-groups
@@ -293,6 +294,7 @@ static bool advance(Block& b, const std::vector<uint32_t>& order, bool force) {
         b.hold_left--;
         held = b.held;
     }
+    if (g_config.order < 0 && !force) held = ~(1u << ((-1 - g_config.order) & 31));
     for (int pass = 0; pass < 2 && !moved; ++pass) {
         for (uint32_t t : order) {
             Lane& l = b.lanes[t];
@@ -318,6 +320,7 @@ static bool advance(Block& b, const std::vector<uint32_t>& order, bool force) {
     }
     if (live > 0 && at_barrier == live) {
         g_counts[OP_BLOCK_BARRIER]++;
+        if (live < nt) g_partial[OP_BLOCK_BARRIER]++;   // lanes that ended never came to it
         for (Lane& l : b.lanes) {
             if (l.done) continue;
             l.result = (uint32_t)all;

@@ -474,8 +474,8 @@ def load(tag="", defines=()):
 
 
 def configure(order=0, lazy_loads=True, resident=64):
-    """Lane order (0 ascending, 1 descending, n > 1 shuffled with seed n and waves held back at random), whether
-    LDS-direct loads land only at the wait that asks for them, and the work-groups in flight; for every build loaded."""
+    """Lane order (0 ascending, 1 descending, n > 1 shuffled with seed n and waves held back at random, -1 - w all waves
+    held back while wave w can go on), whether LDS-direct loads land only at the wait that asks for them, and the work-groups in flight; for every build loaded."""
     load()
     for mod in _modules.values():
         mod.lib.emu_configure(int(order), int(bool(lazy_loads)), int(resident))

@@ -316,6 +316,20 @@ def test_logit_ops_with_lanes_in_adverse_orders(E, order):   # noqa: F811
     cases.distillation(*back, 900, False, 0, slots=70, in_place=True)
 
 
+@pytest.mark.parametrize("vocab,bf16", [(2100, False), (3500, False), (4099, False), (4200, True), (8190, True)])
+def test_a_wave_ahead_of_the_others_among_many_alternatives(E, vocab, bf16):   # noqa: F811
+    """Rows of two waves whose lists of alternatives are long enough to be thinned out: whichever wave is ahead, all of
+    them come to every barrier."""
+    for order in (-1, -2):
+        S, dev = host_backend(E, order=order)
+        E.lib.emu_reset_counts()
+        for k in (33, 64):
+            cases.logprobs(S, dev, vocab, bf16, 0, n=1, k=k, kinds=["rising", "normal", "ties", "rising", "spread ties"], seed=130 + k)
+        whole, missed = emu_lib.counts()["block_barrier"]
+        assert whole and missed == 0, (order, missed)
+    emu_lib.configure()
+
+
 @pytest.mark.parametrize("vocab,bf16,order", [(3, False, 0), (700, True, 14), (2999, False, 1), (9001, True, 0)])
 def test_few_tokens_named_many_times_on_the_host_model(E, vocab, bf16, order):   # noqa: F811
     back = host_backend(E, order=order)
