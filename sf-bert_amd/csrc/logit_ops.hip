@@ -1377,7 +1377,8 @@ __global__ __launch_bounds__(THREADS) void logit_gradient_kernel(GradParams p) {
     T* const d = (T*)p.d_logits + row * p.stride;
     const float m = p.stats[2 * row], l = p.stats[2 * row + 1];
     const float ent = ENTROPY ? -p.scale * p.d_entropy[row] : 0.f, H = ENTROPY ? p.entropy[row] : 0.f;
-    const float w = TEACHER ? p.d_loss[row] / (p.scale * p.scale) : 0.f;
+    const float w = TEACHER ? p.d_loss[row] / p.scale : 0.f;
+    const float factor = TEACHER ? 1.f : p.scale;   // (what a teacher's coefficients are multiplied by is in w)
     if (l == -kInf || (TEACHER && w == 0.f)) {
         write_zeros<T, THREADS>(span, s, d);
         return;
@@ -1430,8 +1431,8 @@ __global__ __launch_bounds__(THREADS) void logit_gradient_kernel(GradParams p) {
         named.total(slots, p.n, s.e0, s.e1);
     }
     RowGrad g;
-    g.set(m, l, p.c, -p.scale * C, ent, H);
-    named.template finish<ENTROPY>(span, g, p.scale);
+    g.set(m, l, p.c, -factor * C, ent, H);
+    named.template finish<ENTROPY>(span, g, factor);
     __syncthreads();
     write_gradient<T, ENTROPY>(span, s, d, g, [&](auto f) { held.each(s, t, f); });
     __syncthreads();
@@ -1535,16 +1536,16 @@ __global__ __launch_bounds__(THREADS, 4) void distill_kernel(DistillParams p) {
         if (p.stats) { p.stats[2 * row] = r.m; p.stats[2 * row + 1] = l; }
     }
     if (!GRAD) return;
-    const float w = p.d_loss[row] / (p.scale * p.scale);
+    const float w = p.d_loss[row] / p.scale;   // (d_loss / scale^2, the coefficients' size, may pass the largest fp32)
     if (!some || w == 0.f || l == -kInf) {
         write_zeros<T, THREADS>(span, s, d);
         return;
     }
     RowGrad g;
-    g.set(r.m, l, p.c, p.scale * w, 0.f, 0.f);
+    g.set(r.m, l, p.c, w, 0.f, 0.f);
 #pragma unroll
     for (uint32_t i = 0; i < named.ROUNDS; ++i)
-        if (named.id[i] >= 0) named.value[i] = fmaf(-p.scale * w, named.value[i], g.template at<false>(LogitVec<T>::value(logits.x[i])));
+        if (named.id[i] >= 0) named.value[i] = fmaf(-w, named.value[i], g.template at<false>(LogitVec<T>::value(logits.x[i])));
     if (!NV) __syncthreads();   // (a streamed row is read again, its named logits have been)
     write_gradient<T, false>(span, s, d, g, [&](auto f) {
         if (NV) held.each(s, t, f);

@@ -448,6 +448,30 @@ def far_from_zero(S, dev, vocab, bf16, value, scale, workspace=None):
     distillation(S, dev, vocab, bf16, 0, slots=6, scale=scale, workspace=workspace, kinds=kinds, seed=123)
 
 
+def large_weights(S, dev, vocab, bf16, scale, weight, workspace=None, slots=9):
+    """Gradients d_loss / scale (p - q) that are ordinary numbers where d_loss / scale^2 is past the largest fp32."""
+    rng = np.random.default_rng(140)
+    x = (rng.standard_normal((5, vocab)) * 2 / scale).astype(np.float32)
+    x = round_bf16(x) if bf16 else x
+    ids = rng.integers(0, vocab, (5, slots)).astype(np.int32)
+    ids[:, 1] = ids[:, 0]
+    z = (rng.standard_normal((5, slots)) * 2 / scale).astype(np.float32)
+    w = (np.float64(weight) * (1 + rng.random(5))).astype(np.float32)
+    w[3] = 0.0
+    _, lp, q = plain_distill(x, ids, z, scale)
+    want = plain_gradient(x, lp, ids, -q * (w / np.float64(scale) ** 2)[:, None], None, scale)
+    assert np.isfinite(want.astype(np.float32)).all()
+    tol = gradient_tol(x, scale, lp, np.abs(w) / scale, want, bf16)
+    # named entries: q's own error, 5 u |t| + (slots + 40) u relative, |t| <= 40
+    named = np.zeros(want.shape)
+    np.put_along_axis(named, ids.astype(np.int64), 1.0, 1)
+    tol = tol + (U * (5 * 40 + slots + 40) * np.abs(w) / scale)[:, None] * named
+    t, tid, tz, tw = dev(x, bf16), dev(ids), dev(z), dev(w)
+    got = S.distillation_loss(t, tid, tz, scale=scale, d_loss=tw, workspace=workspace)
+    same(host(got["d_logits"]), want, tol, "together")
+    same(host(S.distillation_loss_backward(t, tid, tz, got["stats"], tw, scale=scale)), want, tol, "apart")
+
+
 def refusals(S, dev):
     """Calls that are turned away, with the status that says why."""
     import pytest

@@ -131,6 +131,18 @@ def test_logits_far_from_zero_on_the_device(vocab, bf16, value, scale):
     cases.far_from_zero(S, dev, vocab, bf16, value, scale, workspace=torch.zeros(S.LOGIT_WORKSPACE_BYTES, dtype=torch.uint8, device="cuda"))
 
 
+LARGE_WEIGHTS = [(1e-4, 1e33), (1e-3, 5e33)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale,weight", LARGE_WEIGHTS)
+@pytest.mark.parametrize("vocab,bf16", [(300, True), (3000, False), (9001, False), (70001, False), (140001, True)])
+def test_large_weights_on_the_device(vocab, bf16, scale, weight):
+    S, dev = device_backend()
+    cases.large_weights(S, dev, vocab, bf16, scale, weight)
+    cases.large_weights(S, dev, vocab, bf16, scale, weight, workspace=torch.zeros(S.LOGIT_WORKSPACE_BYTES, dtype=torch.uint8, device="cuda"))
+
+
 @pytest.mark.gpu
 def test_teacher_to_student_on_the_device():
     cases.teacher_to_student(*device_backend())
@@ -368,6 +380,13 @@ def test_far_masks_on_the_host_model(E, vocab, bf16, mask, scale):   # noqa: F81
 def test_logits_far_from_zero_on_the_host_model(E, vocab, bf16, value, scale):   # noqa: F811
     S, dev = host_backend(E)
     cases.far_from_zero(S, dev, vocab, bf16, value, scale, workspace=dev(np.zeros(S.LOGIT_WORKSPACE_BYTES, np.uint8)) if vocab > 9000 else None)
+
+
+@pytest.mark.parametrize("scale,weight", LARGE_WEIGHTS)
+@pytest.mark.parametrize("vocab,bf16", [(300, True), (3000, False), (9001, False), (70001, False)])
+def test_large_weights_on_the_host_model(E, vocab, bf16, scale, weight):   # noqa: F811
+    S, dev = host_backend(E)
+    cases.large_weights(S, dev, vocab, bf16, scale, weight, workspace=dev(np.zeros(S.LOGIT_WORKSPACE_BYTES, np.uint8)) if vocab > 9000 else None)
 
 
 def test_teacher_to_student_on_the_host_model(E):   # noqa: F811
