@@ -6,6 +6,8 @@
 #include <sys/mman.h>
 
 #include <map>
+#include <set>
+#include <string>
 #include <vector>
 
 extern "C" void emu_switch(void** save_sp, void* load_sp);
@@ -61,6 +63,7 @@ struct Config {
 static Config g_config;
 static bool g_polling;   // some lane sleeps in a polling loop: what it waits for may be a work-group not yet started
 static uint64_t g_counts[OP_KINDS], g_partial[OP_KINDS];
+static std::set<std::string> g_launched;
 static hipError_t g_error = hipSuccess;
 static char g_message[256];
 
@@ -394,7 +397,8 @@ static void free_block(Block* b) {
     delete b;
 }
 
-void launch(dim3 grid, dim3 block, size_t, hipStream_t, const std::function<void()>& body) {
+void launch(dim3 grid, dim3 block, size_t, hipStream_t, const std::function<void()>& body, const char* kernel) {
+    g_launched.insert(kernel);
     const uint64_t total = (uint64_t)grid.x * grid.y * grid.z;
     const uint32_t nt = block.x * block.y * block.z;
     if (total == 0 || nt == 0 || nt > 1024 || nt % 64 != 0) {   // the model runs whole waves
@@ -461,6 +465,13 @@ void emu_configure(int order, int lazy_loads, int resident) {
 void emu_reset_counts() {
     memset(emu::g_counts, 0, sizeof emu::g_counts);
     memset(emu::g_partial, 0, sizeof emu::g_partial);
+    emu::g_launched.clear();
+}
+const char* emu_launched() {
+    static std::string names;
+    names.clear();
+    for (const std::string& n : emu::g_launched) names += n + ";";
+    return names.c_str();
 }
 uint64_t emu_count(int op) { return op >= 0 && op < emu::OP_KINDS ? emu::g_counts[op] : 0; }
 uint64_t emu_partial_count(int op) { return op >= 0 && op < emu::OP_KINDS ? emu::g_partial[op] : 0; }

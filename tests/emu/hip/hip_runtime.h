@@ -86,7 +86,7 @@ dim3 block_dim();
 dim3 grid_dim();
 void wait(int op);   // gives the processor back until the scheduler has executed the lane's operation
 void* lds_alloc(const void* site, size_t bytes, size_t align);
-void launch(dim3 grid, dim3 block, size_t shared, hipStream_t stream, const std::function<void()>& body);
+void launch(dim3 grid, dim3 block, size_t shared, hipStream_t stream, const std::function<void()>& body, const char* kernel);
 hipError_t last_error();
 
 void global_load_lds_dwordx4(uint32_t m0, uint32_t voffset, uint64_t sbase, int inst_offset);

@@ -3,7 +3,8 @@
 The .hip files are compiled as they are, as plain C++ against tests/emu/hip/hip_runtime.h, after a textual rewrite of
 the three things that are not C++:
 
-* ``kernel<<<grid, block, shared, stream>>>(args);``  ->  ``emu::launch(grid, block, shared, stream, [=]() { kernel(args); });``
+* ``kernel<<<grid, block, shared, stream>>>(args);``  ->  ``emu::launch(grid, block, shared, stream, [=]() { kernel(args); },
+  "kernel");``
 * ``__shared__ T name[N];``  ->  a reference into the work-group's LDS arena
 * ``asm volatile(...)``  ->  the model's function for the instructions it contains; an instruction sequence this
   file does not know stops the build, so a kernel change cannot silently leave the model behind.
@@ -216,8 +217,9 @@ def rewrite(text, name):
             paren += 1
         assert text[paren] == "(", (name, text[at:at + 80])
         end = _balanced(text, paren)
-        out += text[pos:start] + "emu::launch(%s, [=]() { %s(%s); })" % (text[at + 3:close], text[start:at].strip(),
-                                                                      text[paren + 1:end - 1])
+        kernel = text[start:at].strip()
+        out += text[pos:start] + 'emu::launch(%s, [=]() { %s(%s); }, "%s")' % (text[at + 3:close], kernel, text[paren + 1:end - 1],
+                                                                            " ".join(kernel.split()))
         pos = end
     text = out + text[pos:]
     return text
@@ -467,6 +469,7 @@ def load(tag="", defines=()):
     lib.emu_guarded_alloc.restype = C.c_void_p
     lib.emu_guarded_alloc.argtypes = [C.c_size_t]
     lib.emu_message.restype = C.c_char_p
+    lib.emu_launched.restype = C.c_char_p
     lib.emu_count.restype = C.c_uint64
     lib.emu_partial_count.restype = C.c_uint64
     _modules[tag] = mod
@@ -484,6 +487,11 @@ def configure(order=0, lazy_loads=True, resident=64):
 def counts():
     lib = load().lib
     return {name: (int(lib.emu_count(i)), int(lib.emu_partial_count(i))) for i, name in enumerate(OPS)}
+
+
+def launched():
+    """The kernels launched since emu_reset_counts(), as the sources write them (a macro's parameters by their names)."""
+    return set(load().lib.emu_launched().decode().split(";")) - {""}
 
 
 def message():

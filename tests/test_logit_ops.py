@@ -95,6 +95,27 @@ def test_alternatives_behind_masks_and_among_ties_on_the_device(vocab, bf16):
         cases.logprobs(S, dev, vocab, bf16, 3, n=1, k=k, kinds=cases.MASKS_AND_TIES, seed=91 + k, workspace=ws, repeat=2)
 
 
+# the kernels a distillation's loss and gradient come from in one launch, by the largest number of 16-byte vectors in a row
+GRADIENT_SHAPES = [(64, "64, 1"), (256, "64, 4"), (512, "64, 8"), (1024, "128, 8"), (2048, "256, 8"), (4096, "512, 8"),
+                   (8192, "512, 16"), (12288, "512, 24"), (16384, "1024, 16"), (20000, "1024, 0")]
+
+
+def at_the_limit(vecs, bf16, over):
+    """The odd vocabulary closest to the limit that still is (over: no longer is) within it."""
+    n = 8 if bf16 else 4
+    return vecs * n + (n + 1 if over else n - 1)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("vecs", [vecs for vecs, _ in GRADIENT_SHAPES])
+def test_every_shape_of_the_distillation_gradient_on_the_device(vecs, bf16):
+    for over in (False, True):
+        vocab = at_the_limit(vecs, bf16, over)
+        cases.distillation(*device_backend(), vocab, bf16, 0, slots=9, seed=150)
+        cases.distillation(*device_backend(), vocab, bf16, 0, slots=130, teacher_bf16=True, in_place=True, seed=151, few=True)
+
+
 FAR_APART = [(11, False), (200, True), (1000, False), (2500, False), (9001, True), (40000, False)]
 
 
@@ -340,6 +361,24 @@ def test_a_wave_ahead_of_the_others_among_many_alternatives(E, vocab, bf16):   #
         whole, missed = emu_lib.counts()["block_barrier"]
         assert whole and missed == 0, (order, missed)
     emu_lib.configure()
+
+
+@pytest.mark.parametrize("bf16", [False, True])
+@pytest.mark.parametrize("at", range(len(GRADIENT_SHAPES)))
+def test_every_shape_of_the_distillation_gradient_on_the_host_model(E, at, bf16):   # noqa: F811
+    S, dev = host_backend(E)
+    vecs, shape = GRADIENT_SHAPES[at]
+    some = ["normal", "lowest", "ties", "late peak", "masked", "peaked", "normal"]
+    for over in (False, True):
+        expected = shape if not over else GRADIENT_SHAPES[min(at + 1, len(GRADIENT_SHAPES) - 1)][1]
+        vocab = at_the_limit(vecs, bf16, over)
+        E.lib.emu_reset_counts()
+        S.distillation_loss(dev(cases.matrix(vocab, 1, bf16, ["normal"]), bf16), dev(np.zeros((1, 3), np.int32)), dev(np.zeros((1, 3), np.float32)),
+                            d_loss=dev(np.ones(1, np.float32)))
+        # (the two the sources write out: with the gradient only, and with the loss alone too)
+        assert len(emu_lib.launched()) == 1 and emu_lib.launched() <= {"distill_kernel<T, %s, %s>" % (expected, g) for g in ("GRAD", "true")}
+        cases.distillation(S, dev, vocab, bf16, 0, slots=9, seed=150, kinds=some)
+        cases.distillation(S, dev, vocab, bf16, 0, slots=130, teacher_bf16=True, in_place=True, seed=151, few=True, kinds=some)
 
 
 @pytest.mark.parametrize("vocab,bf16,order", [(3, False, 0), (700, True, 14), (2999, False, 1), (9001, True, 0)])
