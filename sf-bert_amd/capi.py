@@ -931,7 +931,7 @@ def _logit_rows(logits):
         raise SfbError(4, "logits of %d dimensions" % logits.dim())
     rows, vocab = logits.shape
     stride, step = logits.stride()
-    if rows == 1 and stride < vocab:
+    if rows == 1:   # (its distance to the next row is that of a view, and means nothing)
         stride = vocab
     if rows == 0 or vocab == 0 or stride < vocab or (step != 1 and vocab > 1):
         raise SfbError(4, "logits of shape %s with strides %s" % (tuple(logits.shape), logits.stride()))
@@ -1016,7 +1016,8 @@ def token_logprobs(logits, tokens=None, top_k=0, scale=1.0, entropy=False, works
 
 def token_logprobs_backward(logits, tokens, stats, d_logprob=None, entropy=None, d_entropy=None, scale=1.0, out=None):
     """d_logits of sum d_logprob * logprob + sum d_entropy * entropy (sfb_token_logprobs_backward), from token_logprobs'
-    stats (and entropy, where d_entropy is given); out may be the logits themselves."""
+    stats (and entropy, where d_entropy is given).  out may be the logits themselves; the gradient's rows are as far apart
+    as theirs, so without out a view of one position in every sequence gets a buffer as large as the whole logits."""
     import torch
     code, rows, vocab, stride = _logit_rows(logits)
     stream = _stream_for(logits, tokens, stats, d_logprob, entropy, d_entropy, out)
@@ -1047,7 +1048,8 @@ def distillation_loss(logits, teacher_ids, teacher_logits, scale=1.0, d_loss=Non
     """Divergence of softmax(scale * logits) from a teacher's top logits, per row (sfb_distillation_loss).  teacher_ids
     int32 and teacher_logits fp32 or bf16 [rows, slots]; ids outside the vocabulary are unused slots.  Returns a dict:
     row_loss [rows], stats [rows, 2] (parts of one allocation), and with d_loss [rows] (the gradient of each row's loss) also d_logits, written
-    to out (which may be the logits themselves) if given.  workspace as for token_logprobs."""
+    to out (which may be the logits themselves) if given, else to rows as far apart as the logits'.  workspace as for
+    token_logprobs."""
     import torch
     code, rows, vocab, stride = _logit_rows(logits)
     stream = _stream_for(logits, teacher_ids, teacher_logits, d_loss, out, workspace)
@@ -1069,7 +1071,8 @@ def distillation_loss(logits, teacher_ids, teacher_logits, scale=1.0, d_loss=Non
 
 
 def distillation_loss_backward(logits, teacher_ids, teacher_logits, stats, d_loss, scale=1.0, out=None):
-    """d_logits of sum d_loss * row_loss from distillation_loss's stats (sfb_distillation_loss_backward)."""
+    """d_logits of sum d_loss * row_loss from distillation_loss's stats (sfb_distillation_loss_backward); out as for
+    token_logprobs_backward."""
     import torch
     code, rows, vocab, stride = _logit_rows(logits)
     stream = _stream_for(logits, teacher_ids, teacher_logits, stats, d_loss, out)

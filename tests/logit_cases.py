@@ -472,6 +472,23 @@ def large_weights(S, dev, vocab, bf16, scale, weight, workspace=None, slots=9):
     same(host(S.distillation_loss_backward(t, tid, tz, got["stats"], tw, scale=scale)), want, tol, "apart")
 
 
+def one_row_of_many(S, dev, rows=1, apart=64, vocab=50):
+    """Rows far apart (one position of every sequence): the gradient has their distance, but a single row has none."""
+    base = dev(np.random.default_rng(150).standard_normal((rows, apart * vocab)).astype(np.float32))
+    x = base[:, (apart - 2) * vocab:(apart - 1) * vocab]
+    assert x.stride(0) == apart * vocab
+    tok, w = dev(np.arange(rows, dtype=np.int32)), dev(np.ones(rows, np.float32))
+    lp = S.token_logprobs(x, tok)
+    d = S.token_logprobs_backward(x, tok, lp["stats"], d_logprob=w)
+    both = S.distillation_loss(x, tok[:, None], w[:, None], d_loss=w)
+    for got in (d, both["d_logits"], S.distillation_loss_backward(x, tok[:, None], w[:, None], both["stats"], w)):
+        assert got.shape == x.shape
+        assert got.untyped_storage().nbytes() == 4 * vocab * (1 if rows == 1 else rows * apart)
+    p = np.exp(plain_log_softmax(host(x).astype(np.float32), 1.0))
+    p[np.arange(rows), np.arange(rows)] -= 1
+    assert np.abs(host(d) + p).max() < 1e-6 and np.abs(host(both["d_logits"]) - p).max() < 1e-6
+
+
 def refusals(S, dev):
     """Calls that are turned away, with the status that says why."""
     import pytest

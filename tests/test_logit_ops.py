@@ -175,6 +175,12 @@ def test_parts_left_out_on_the_device():
 
 
 @pytest.mark.gpu
+def test_rows_far_apart_on_the_device():
+    cases.one_row_of_many(*device_backend())
+    cases.one_row_of_many(*device_backend(), rows=3)
+
+
+@pytest.mark.gpu
 @pytest.mark.needs_device
 def test_host_tensors_are_refused():
     S, dev = device_backend()
@@ -434,6 +440,11 @@ def test_teacher_to_student_on_the_host_model(E):   # noqa: F811
 
 def test_parts_left_out_on_the_host_model(E):   # noqa: F811
     cases.parts_left_out(*host_backend(E))
+
+
+def test_rows_far_apart_on_the_host_model(E):   # noqa: F811
+    cases.one_row_of_many(*host_backend(E))
+    cases.one_row_of_many(*host_backend(E), rows=3)
 
 
 def test_refusals_on_the_host_model(E):   # noqa: F811
