@@ -592,7 +592,45 @@ template <typename T, int THREADS, int HELD> struct TopSelect {
         __syncthreads();
         return shared().count;
     }
-    // the exact k largest: those above the k-th largest value, and of those equal to it the lowest-index ones
+    // The k-th largest value, of which it is known that `from` is not above it, digit by digit from the highest: how many
+    // values share the digits so far and have which next one.
+    static __device__ uint32_t kth_largest(const RowSpan<T>& span, const Slice& s, uint32_t k, uint32_t from) {
+        constexpr int BITS = VECTORS >= 256 ? 8 : 6;
+        constexpr uint32_t BINS = 1u << BITS, SHARE = BINS / 16;
+        static_assert(BINS <= VECTORS, "the counts share memory with the vectors");
+        const uint32_t t = threadIdx.x;
+        uint32_t value = 0, left = k;
+        for (int high = 32; high > 0;) {
+            const int low = high > BITS ? high - BITS : 0;
+            const uint32_t known = high == 32 ? 0u : ~0u << high, digits = (1u << (high - low)) - 1;
+            __syncthreads();
+            for (uint32_t i = t; i < BINS; i += THREADS) shared().at[i] = 0;
+            __syncthreads();
+            elements(span, s, [&](uint32_t order, uint32_t j) {
+                if (j < s.e1 && order >= from && ((order ^ value) & known) == 0)
+                    __hip_atomic_fetch_add(&shared().at[order >> low & digits], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                return true;
+            });
+            __syncthreads();
+            if (t < 16) {   // (the list is free: what it held was too much)
+                uint32_t sum = 0;
+                for (uint32_t i = 0; i < SHARE; ++i) sum += shared().at[t * SHARE + i];
+                shared().list[t] = sum;
+            }
+            __syncthreads();
+            uint32_t group = 15, above = 0;
+            for (; group > 0 && above + (uint32_t)shared().list[group] < left; --group) above += (uint32_t)shared().list[group];
+            uint32_t digit = group * SHARE + SHARE - 1;
+            for (; digit > group * SHARE && above + shared().at[digit] < left; --digit) above += shared().at[digit];
+            left -= above;
+            value |= digit << low;
+            high = low;
+        }
+        return value;
+    }
+    // The exact k largest: those above the k-th largest value, and of those equal to it the lowest-index ones.  limit: a
+    // value that k logits reach.  (Reads the slice at most seven times, nine in rows of up to 64 vectors.  4096 rows of
+    // 30522 rising fp32 logits, k = 20: 845 us; 93 where it is not needed.)
     static __device__ void select_exactly(const RowSpan<T>& span, const Slice& s, uint32_t k, uint32_t limit, bool known) {
         if (s.e1 - s.e0 <= k) {
             clear_count();
@@ -603,14 +641,8 @@ template <typename T, int THREADS, int HELD> struct TopSelect {
             __syncthreads();
             return;
         }
-        // (limit given: the k-th largest if fewer than k logits are above it -- a masked vocabulary)
-        if (!known || reaching(span, s, limit + 1) >= k) {
-            limit = 0;
-            for (int bit = 31; bit >= 0; --bit) {
-                const uint32_t next = limit | (1u << bit);
-                if (reaching(span, s, next) >= k) limit = next;
-            }
-        }
+        // (known: limit is the k-th largest if fewer than k logits are above it -- a masked vocabulary)
+        if (!known || reaching(span, s, limit + 1) >= k) limit = kth_largest(span, s, k, limit);
         clear_count();
         elements(span, s, [&](uint32_t order, uint32_t j) {
             if (order > limit) append(order, j);
@@ -923,7 +955,7 @@ __device__ __forceinline__ void finish_collection(const RowSpan<T>& span, const 
         return;
     }
     uint32_t kind = Top::kBetween;
-    const uint32_t limit = nan ? 0u : Top::threshold(r.top, any, k, &kind);
+    const uint32_t limit = Top::threshold(r.top, any, k, &kind);
     auto every = [&](float from) {
         Streamed<T, THREADS>::each(span, s, t, [&](const float (&x)[N], uint32_t base) { Top::scan(x, span.index(base + t), from); });
     };

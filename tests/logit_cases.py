@@ -81,6 +81,13 @@ def logits_of(kind, vocab, rng, bf16):
         x[keep] = kept
     elif kind.startswith("all of "):   # a row whose logits are all masked
         x[:] = float(kind[7:])
+    elif kind == "falling":
+        x = np.linspace(60.0, -60.0, vocab).astype(np.float32)
+    elif kind == "first ones large":   # a vocabulary in the order of its tokens' frequencies
+        x[:700] += 30.0
+    elif kind == "coarse":   # more equal largest logits than any list holds, far fewer than half of the row
+        x = np.floor(np.abs(x))
+        x[vocab // 3:vocab // 3 + 1500] = 20.0
     elif kind.startswith("around "):   # neighbours among the numbers of that size
         x = np.float32(float(kind[7:])) * (1 + rng.integers(0, 4, vocab) * np.float32(2.0 ** -7 if bf16 else 2.0 ** -23))
     return round_bf16(x) if bf16 else x.astype(np.float32)

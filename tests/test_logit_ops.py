@@ -95,6 +95,19 @@ def test_alternatives_behind_masks_and_among_ties_on_the_device(vocab, bf16):
         cases.logprobs(S, dev, vocab, bf16, 3, n=1, k=k, kinds=cases.MASKS_AND_TIES, seed=91 + k, workspace=ws, repeat=2)
 
 
+CLUSTERED = ["rising", "falling", "first ones large", "coarse", "nan", "inf"]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab,bf16", [(70, False), (1000, True), (2999, False), (8190, True), (9001, False), (40000, True), (70001, False), (131072, False)])
+def test_clustered_alternatives_on_the_device(vocab, bf16):
+    S, dev = device_backend()
+    ws = torch.zeros(S.LOGIT_WORKSPACE_BYTES, dtype=torch.uint8, device="cuda")
+    for k in (9, 16, 17, 32, 33, 64):
+        cases.logprobs(S, dev, vocab, bf16, 1, n=1, k=k, kinds=CLUSTERED, seed=160 + k, repeat=2)
+        cases.logprobs(S, dev, vocab, bf16, 0, n=1, k=k, kinds=CLUSTERED, seed=161 + k, repeat=2, workspace=ws)
+
+
 # the kernels a distillation's loss and gradient come from in one launch, by the largest number of 16-byte vectors in a row
 GRADIENT_SHAPES = [(64, "64, 1"), (256, "64, 4"), (512, "64, 8"), (1024, "128, 8"), (2048, "256, 8"), (4096, "512, 8"),
                    (8192, "512, 16"), (12288, "512, 24"), (16384, "1024, 16"), (20000, "1024, 0")]
@@ -367,6 +380,25 @@ def test_a_wave_ahead_of_the_others_among_many_alternatives(E, vocab, bf16):   #
         whole, missed = emu_lib.counts()["block_barrier"]
         assert whole and missed == 0, (order, missed)
     emu_lib.configure()
+
+
+@pytest.mark.parametrize("vocab,bf16", [(2999, False), (8190, True), (9001, False), (40000, True), (70001, False)])
+def test_reads_of_rows_with_clustered_alternatives(E, vocab, bf16):   # noqa: F811
+    """However the largest logits stand together, a row is read a bounded number of times, not once for every bit of a
+    logit: the work-group meets four times for each read, and twice for every step that looks for equal logits."""
+    vecs = vocab // (8 if bf16 else 4)
+    steps = -(-vocab // (128 if vecs <= 1024 else 256 if vecs <= 4096 else 512))
+    S, dev = host_backend(E)
+    tok = dev(np.zeros(1, np.int32))
+    for kind in CLUSTERED:
+        x = dev(cases.matrix(vocab, 7, bf16, [kind]), bf16)
+        for k in (9, 16, 17, 20, 32, 33, 64):
+            E.lib.emu_reset_counts()
+            S.token_logprobs(x, tok, top_k=k)
+            assert emu_lib.counts()["block_barrier"][0] < 4 * 10 + 2 * steps, (kind, k)
+    for k in (9, 17, 64):
+        cases.logprobs(S, dev, vocab, bf16, 1, n=1, k=k, kinds=CLUSTERED, seed=160 + k)
+        cases.logprobs(S, dev, vocab, bf16, 0, n=1, k=k, kinds=CLUSTERED, seed=161 + k, workspace=dev(np.zeros(S.LOGIT_WORKSPACE_BYTES, np.uint8)))
 
 
 @pytest.mark.parametrize("bf16", [False, True])
