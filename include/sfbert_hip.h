@@ -644,12 +644,14 @@ int sfb_softmax_cross_entropy(sfb_stream_t stream, float* loss, float* row_loss,
 
 /* Shared by the four entry points below.  logits [dev] is rows x vocab of dtype (SFB_F32 or SFB_BF16), 16-byte aligned,
  * with rows row_stride >= vocab elements apart (any stride: rows may start at any element; columns from vocab on are
- * neither read nor written); d_logits has the same type, stride and alignment and may be logits itself.  Every result
- * is a function of scale * logits (scale = 1 / temperature, SFB_LOGIT_SCALE_MIN .. SFB_LOGIT_SCALE_MAX), computed in
- * fp32; bf16 gradients are rounded once.  -inf is a masked logit: probability 0, no share of the entropy, gradient 0.
- * A row that holds NaN or +inf gives NaN, a row of nothing but -inf gives log probabilities of -inf, entropy 0 and a
- * zero gradient.  Logits as large as the type's largest and lowest value are ordinary numbers.  Results of one launch
- * do not depend on the order in which threads run: the same inputs give the same bits.
+ * neither read nor written); d_logits has the same type, stride and alignment; it may be logits itself and must not
+ * overlap them otherwise.  Every result is a function of scale * logits (scale = 1 / temperature, SFB_LOGIT_SCALE_MIN ..
+ * SFB_LOGIT_SCALE_MAX), computed in fp32; bf16 gradients are rounded once.  -inf is a masked logit: probability 0, no
+ * share of the entropy, and no gradient but what a token or a slot that names it brings there (the sums in the formulas
+ * below).  A row that holds NaN or +inf gives NaN, a row of nothing but -inf gives log probabilities of -inf, entropy 0
+ * and a zero gradient.  All finite logits, up to the type's largest and lowest value, are ordinary numbers (a mask may be
+ * any of them).  Results of one launch do not depend on the order in which threads run: the same inputs give the same
+ * bits.
  * stats [dev] float[rows][2] (may be NULL): the row's reference logit m and log2 sum_j 2^((x_j - m) scale log2(e)),
  * which the backward entry points take; with s = scale, ln sum_j exp(s x_j) = s m + ln(2) stats[1].
  * rows x the threads of a row (64 to 1024) stay below 2^32, or the call returns SFB_ERR_SHAPE.
@@ -685,7 +687,8 @@ int sfb_token_logprobs_backward(sfb_stream_t stream, void* d_logits, const void*
  * id is outside [0, vocab) is unused (lists of different lengths).  With q = softmax(scale * teacher_logits) over a
  * row's used slots and p = softmax(scale * logits) over the vocabulary,
  *   row_loss[r] = 1 / scale^2 sum_k q_k (ln q_k - ln p[teacher_ids[r][k]])
- * (Kullback-Leibler divergence times the squared temperature).  A token named twice counts with both slots.  A row
+ * (Kullback-Leibler divergence times the squared temperature).  A slot whose q is too small for fp32 counts as one of
+ * probability 0, also where the student's is 0.  A token named twice counts with both slots.  A row
  * without a used slot has loss 0; its logits are not read.
  * d_logits not NULL: also the gradient of sum_r d_loss[r] row_loss[r] (d_loss [dev] float[rows]),
  *   d_logits[r][j] = d_loss[r] / scale ( p_j - sum_{k: teacher_ids[r][k] = j} q_k ),
